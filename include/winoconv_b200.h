@@ -256,6 +256,57 @@ WINOCONV_API int winoconv_backward_weight(const winoconv_desc_t *desc, const voi
                                           float *dbias, void *ws, size_t ws_bytes, void *stream);
 
 /*
+ * Fully connected layers: y = act(x W^T + bias) + residual, and its gradients.  16-bit operands, products and sums in fp32, one
+ * rounding at the end.  Rows of every matrix are contiguous; a stride is the distance of two rows in elements (0: no gap).  The
+ * matrices that the tensor cores read (x, w, dz) start on 16 bytes and have strides that are multiples of 8
+ * (winoconv_pad_rows makes such a copy); the others may lie anywhere.  No scratch but where it is said.
+ *   forward     z = x W^T + bias; y = act(z) + residual.  bias, residual may be NULL.  z (dtype) or z8 with z8_scale (eight bits,
+ *               as winoconv_e4m3_pack writes them) receive the pre-activation where they are not NULL.
+ *   activation  dz = gy act'(z), dbias = sums of its columns.  z or z8 with z8_scale as kept by the forward (neither with
+ *               WINOCONV_ACT_NONE); dz, dbias may be NULL; ws: winoconv_linear_backward_ws bytes where dbias is not NULL.
+ *   data        dx = dz W.
+ *   weight      dW = dz^T x, [out_features][in_features] without gaps, in dw_dtype.
+ * No counterpart in the reference, which has convolutions only.
+ */
+typedef enum winoconv_act {
+  WINOCONV_ACT_NONE = 0,
+  WINOCONV_ACT_RELU = 1,
+  WINOCONV_ACT_GELU = 2,      /* z (1 + erf(z / sqrt 2)) / 2                                     */
+  WINOCONV_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2               */
+  WINOCONV_ACT_SILU = 4       /* z / (1 + exp(-z))                                               */
+} winoconv_act_t;
+typedef struct winoconv_linear_desc {
+  int64_t rows;
+  int32_t in_features, out_features;
+  int32_t dtype;              /* F16 or BF16: x, w, residual, y, z, gy, dz, dx                   */
+  int32_t activation;         /* winoconv_act_t                                                  */
+  int32_t bias_f32;           /* 1: the bias is f32 whatever dtype is                            */
+  int32_t reserved;
+  int64_t x_stride, w_stride, residual_stride, y_stride, z_stride;
+} winoconv_linear_desc_t;
+WINOCONV_API int winoconv_linear_forward(const winoconv_linear_desc_t *desc, const void *x, const void *w, const void *bias, const void *residual,
+                                         void *y, void *z, void *z8, void *z8_scale, void *stream);
+WINOCONV_API int winoconv_linear_backward_ws(const winoconv_linear_desc_t *desc, uint64_t *bytes);
+WINOCONV_API int winoconv_linear_backward_activation(const winoconv_linear_desc_t *desc, const void *gy, int64_t gy_stride, const void *z, const void *z8,
+                                                     const void *z8_scale, void *dz, int64_t dz_stride, void *dbias, int dbias_dtype, void *ws,
+                                                     size_t ws_bytes, void *stream);
+WINOCONV_API int winoconv_linear_backward_data(const winoconv_linear_desc_t *desc, const void *dz, int64_t dz_stride, const void *w, void *dx,
+                                               int64_t dx_stride, void *stream);
+WINOCONV_API int winoconv_linear_backward_weight(const winoconv_linear_desc_t *desc, const void *dz, int64_t dz_stride, const void *x, void *dw,
+                                                 int dw_dtype, void *stream);
+/* x [rows][cols] of 16-bit values -> y [rows][y_stride] (a multiple of 8, y on 16 bytes), zeros from column `cols` on. */
+WINOCONV_API int winoconv_pad_rows(const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int32_t cols, void *stream);
+
+/*
+ * Activations kept in eight bits: 32 neighbours of a row share a power of two 2^e, the smallest (from 2^-127 on) that brings the
+ * largest finite magnitude among them within 448, and are rounded to e4m3 (half to even).  q [rows][cols] without gaps; scale
+ * [rows][ceil(cols / 32)] holds e + 127.  Infinities and NaN are kept as NaN.  unpack gives q 2^e, cut to dtype's finite range:
+ * the values have four significant bits and need no other rounding (but below dtype's subnormals).
+ */
+WINOCONV_API int winoconv_e4m3_pack(int dtype, const void *x, int64_t x_stride, int64_t rows, int32_t cols, void *q, void *scale, void *stream);
+WINOCONV_API int winoconv_e4m3_unpack(int dtype, const void *q, const void *scale, int64_t rows, int32_t cols, void *x, int64_t x_stride, void *stream);
+
+/*
  * The per-position batched GEMM on its own: m[p][t][k] = sum_c v[p][t][c] * u[p][k][c],
  * fp32 accumulate.  v [positions][tiles][c_pad], u [positions][k_out][c_pad] in `dtype`,
  * m [positions][tiles][k_out] in `product_dtype`.  c_pad must be a multiple of 8.

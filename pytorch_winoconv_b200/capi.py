@@ -31,6 +31,8 @@ EXPORTED_SYMBOLS = (
     "winoconv_concat", "winoconv_add", "winoconv_read_device_error", "winoconv_probe_mma_rate",
     "winoconv_filter_transform_from", "winoconv_backward_plan", "winoconv_backward_filter_transform",
     "winoconv_backward_data", "winoconv_backward_weight", "winoconv_to_channels_last", "winoconv_to_channels_first",
+    "winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation", "winoconv_linear_backward_data",
+    "winoconv_linear_backward_weight", "winoconv_pad_rows", "winoconv_e4m3_pack", "winoconv_e4m3_unpack",
 )
 
 
@@ -49,6 +51,12 @@ class PlanInfo(Structure):
                 ("input_ws_bytes", c_uint64), ("product_ws_bytes", c_uint64), ("input_ws_bytes_min", c_uint64),
                 ("product_ws_bytes_min", c_uint64), ("block_tiles", c_int64), ("direct_flops", c_double),
                 ("gemm_flops", c_double), ("algorithmic_bytes", c_double)]
+
+
+class LinearDesc(Structure):
+    _fields_ = [("rows", c_int64), ("in_features", c_int32), ("out_features", c_int32), ("dtype", c_int32), ("activation", c_int32),
+                ("bias_f32", c_int32), ("reserved", c_int32), ("x_stride", c_int64), ("w_stride", c_int64),
+                ("residual_stride", c_int64), ("y_stride", c_int64), ("z_stride", c_int64)]
 
 
 class WinoconvError(RuntimeError):
@@ -92,6 +100,19 @@ def lib() -> ctypes.CDLL:
     L.winoconv_probe_mma_rate.argtypes = [c_int, c_int, c_int, c_int, c_int, POINTER(ctypes.c_float),
                                           POINTER(ctypes.c_float), c_void_p]
     L.winoconv_probe_mma_rate.restype = c_int
+    L.winoconv_linear_forward.argtypes = [POINTER(LinearDesc)] + [c_void_p] * 9
+    L.winoconv_linear_backward_ws.argtypes = [POINTER(LinearDesc), POINTER(c_uint64)]
+    L.winoconv_linear_backward_activation.argtypes = [POINTER(LinearDesc), c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                                      c_int64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]
+    L.winoconv_linear_backward_data.argtypes = [POINTER(LinearDesc), c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
+    L.winoconv_linear_backward_weight.argtypes = [POINTER(LinearDesc), c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]
+    L.winoconv_pad_rows.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p]
+    L.winoconv_e4m3_pack.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p]
+    L.winoconv_e4m3_unpack.argtypes = [c_int, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]
+    for name in ("winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation",
+                 "winoconv_linear_backward_data", "winoconv_linear_backward_weight", "winoconv_pad_rows", "winoconv_e4m3_pack",
+                 "winoconv_e4m3_unpack"):
+        getattr(L, name).restype = c_int
     for name in ("winoconv_plan", "winoconv_plan_pieces", "winoconv_filter_transform", "winoconv_forward",
                  "winoconv_forward_timed", "winoconv_forward_static", "winoconv_gemm_batched", "winoconv_split",
                  "winoconv_concat", "winoconv_add", "winoconv_read_device_error"):

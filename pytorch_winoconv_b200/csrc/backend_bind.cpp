@@ -3,6 +3,7 @@
 
 #include "backend_ops.h"
 #include "conv_module.h"
+#include "linear_module.h"
 
 namespace py = pybind11;
 
@@ -19,6 +20,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_dwm_output_block", &set_dwm_output_block);
   m.def("get_dwm_output_block", &get_dwm_output_block);
   m.def("conv_call", &conv_call, py::call_guard<py::gil_scoped_release>());
+  m.def("linear_call", &linear_call, py::call_guard<py::gil_scoped_release>());
+  m.def("e4m3_pack", &e4m3_pack, py::call_guard<py::gil_scoped_release>());
+  m.def("e4m3_unpack", [](const at::Tensor &q, const at::Tensor &scale, const py::object &dtype) {
+    const at::ScalarType type = torch::python::detail::py_object_to_dtype(dtype);
+    py::gil_scoped_release release;
+    return e4m3_unpack(q, scale, type);
+  });
   py::class_<ConvRunner, c10::intrusive_ptr<ConvRunner>>(m, "ConvRunner")
       .def(py::init<int64_t, std::vector<int64_t>, std::vector<int64_t>, int64_t, int64_t, bool, bool, int64_t, int64_t>())
       .def("forward", &ConvRunner::forward, py::call_guard<py::gil_scoped_release>())

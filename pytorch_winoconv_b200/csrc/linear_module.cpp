@@ -1,0 +1,274 @@
+#include "linear_module.h"
+
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+
+#include <vector>
+
+#include "winoconv_b200.h"
+
+namespace {
+
+int code_of(at::ScalarType t) {
+  switch (t) {
+    case at::kFloat: return WINOCONV_F32;
+    case at::kHalf: return WINOCONV_F16;
+    case at::kBFloat16: return WINOCONV_BF16;
+    default: return -1;
+  }
+}
+bool is16(const at::Tensor &t) { return t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16; }
+void check_abi(int st, const char *what) {
+  if (st == WINOCONV_OK) return;
+  char buf[1024];
+  winoconv_last_error(buf, sizeof buf);
+  TORCH_CHECK(false, what, " failed (", winoconv_status_string(st), "): ", buf);
+}
+void *stream_of() { return (void *)at::cuda::getCurrentCUDAStream().stream(); }
+at::TensorOptions plain(const at::Tensor &like) { return like.options().requires_grad(false); }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Row stride of a matrix whose rows are contiguous; 0 where they are not or overlap.
+int64_t row_stride(const at::Tensor &t) {
+  const int64_t cols = t.size(1);
+  if (cols > 1 && t.stride(1) != 1) return 0;
+  if (t.size(0) == 1) return round8(cols);      // of no meaning
+  return t.stride(0) >= cols ? t.stride(0) : 0;
+}
+// A matrix with contiguous rows.
+at::Tensor with_rows(const at::Tensor &t) { return row_stride(t) ? t : t.contiguous(); }
+// A matrix as the tensor cores' loads want it: rows on 16 bytes.  Else a copy with padded rows (of which the first cols are seen).
+at::Tensor operand(const at::Tensor &in) {
+  const at::Tensor t = with_rows(in);
+  if (row_stride(t) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0) return t;
+  const int64_t rows = t.size(0), cols = t.size(1), ld = round8(cols);
+  at::Tensor out = at::empty({rows, ld}, plain(t));
+  check_abi(winoconv_pad_rows(t.data_ptr(), rows == 1 ? cols : row_stride(t), out.data_ptr(), ld, rows, (int32_t)cols, stream_of()), "winoconv_pad_rows");
+  return out.narrow(1, 0, cols);
+}
+// Its stride for the C ABI.
+int64_t ld_of(const at::Tensor &t) { return row_stride(t); }
+
+at::Tensor as_rows(const at::Tensor &t, int64_t cols) { return t.reshape({-1, cols}); }
+
+struct Shape {
+  int64_t rows, k, n;
+};
+winoconv_linear_desc_t describe(const Shape &s, at::ScalarType type, int act) {
+  winoconv_linear_desc_t d = {};
+  TORCH_CHECK(s.rows <= 0x7fffffffLL && s.k <= 0x7fffffffLL && s.n <= 0x7fffffffLL, "linear: matrix too large");
+  d.rows = s.rows;
+  d.in_features = (int32_t)s.k;
+  d.out_features = (int32_t)s.n;
+  d.dtype = code_of(type);
+  d.activation = act;
+  return d;
+}
+
+// What a layer keeps for its backward pass: x and z, or their eight bits with the scales.
+struct Kept {
+  at::Tensor x, x_scale, z, z_scale;
+};
+
+at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &residual, int act, bool pack, bool keep_x,
+                   bool keep_z, Kept *kept) {
+  const at::ScalarType type = x.scalar_type();
+  const int64_t k = weight.size(1), n = weight.size(0);
+  at::Tensor x2 = as_rows(x, k);
+  const Shape s{x2.size(0), k, n};
+  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+  sizes.back() = n;
+  at::Tensor y = at::empty(sizes, plain(x));
+  if (kept && keep_x) {
+    if (pack) std::tie(kept->x, kept->x_scale) = e4m3_pack(x2);
+    else kept->x = x;
+  }
+  if (kept && keep_z) {
+    if (pack) {
+      kept->z = at::empty({s.rows, n}, plain(x).dtype(at::kFloat8_e4m3fn));
+      kept->z_scale = at::empty({s.rows, (n + 31) / 32}, plain(x).dtype(at::kFloat8_e8m0fnu));
+    } else kept->z = at::empty({s.rows, n}, plain(x));
+  }
+  if (s.rows == 0) return y;
+  x2 = operand(x2);
+  const at::Tensor w = operand(weight.scalar_type() == type ? weight : weight.to(type));
+  const at::Tensor b = bias.defined() ? bias.contiguous() : bias;
+  const at::Tensor r = residual.defined() ? with_rows(as_rows(residual, n)) : residual;
+  winoconv_linear_desc_t d = describe(s, type, act);
+  d.bias_f32 = b.defined() && b.scalar_type() == at::kFloat;
+  d.x_stride = ld_of(x2);
+  d.w_stride = ld_of(w);
+  if (r.defined() && s.rows > 1) d.residual_stride = ld_of(r);
+  const bool z = kept && keep_z;
+  check_abi(winoconv_linear_forward(&d, x2.data_ptr(), w.data_ptr(), b.defined() ? b.data_ptr() : nullptr, r.defined() ? r.data_ptr() : nullptr, y.data_ptr(),
+                                    z && !pack ? kept->z.data_ptr() : nullptr, z && pack ? kept->z.data_ptr() : nullptr,
+                                    z && pack ? kept->z_scale.data_ptr() : nullptr, stream_of()),
+            "winoconv_linear_forward");
+  return y;
+}
+
+struct LinearFn : public torch::autograd::Function<LinearFn> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias,
+                            const std::optional<at::Tensor> &residual, int64_t act, bool pack) {
+    const bool nx = x.requires_grad(), nw = weight.requires_grad(), nb = bias && bias->requires_grad();
+    Kept kept;
+    at::Tensor y;
+    {
+      at::AutoDispatchBelowADInplaceOrView no_graph;
+      y = ::forward(x, weight, bias ? *bias : at::Tensor(), residual ? *residual : at::Tensor(), (int)act, pack, nw,
+                    act != WINOCONV_ACT_NONE && (nx || nw || nb), &kept);
+    }
+    ctx->save_for_backward({kept.x, kept.x_scale, kept.z, kept.z_scale, nx ? weight : at::Tensor()});
+    ctx->saved_data["sizes"] = x.sizes().vec();
+    ctx->saved_data["w_sizes"] = weight.sizes().vec();
+    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(), bias ? (int64_t)bias->scalar_type() : -1, act, pack};
+    ctx->saved_data["given"] = std::vector<int64_t>{bias.has_value(), residual.has_value()};
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(6);
+    if (!grads[0].defined()) return out;
+    TORCH_CHECK(!at::GradMode::is_enabled(), "linear: the gradients are not differentiable again (create_graph=True)");
+    at::AutoDispatchBelowADInplaceOrView no_graph;
+    const auto saved = ctx->get_saved_variables();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector(), w_sizes = ctx->saved_data["w_sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector(),
+               given = ctx->saved_data["given"].toIntVector();
+    const auto type = (at::ScalarType)types[0], w_type = (at::ScalarType)types[1];
+    const int act = (int)types[3];
+    const bool pack = types[4] != 0;
+    // numbered by the tensors among the arguments of apply
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = given[0] && ctx->needs_input_grad(2),
+               nr = given[1] && ctx->needs_input_grad(2 + given[0]);
+    const at::Tensor &gy = grads[0];
+    c10::cuda::CUDAGuard guard(gy.device());
+    if (nr) out[3] = gy;
+    if (!nx && !nw && !nb) return out;
+    const int64_t n = w_sizes[0], k = w_sizes[1];
+    at::Tensor g = with_rows(as_rows(gy, n));
+    const Shape s{g.size(0), k, n};
+    at::Tensor dx, dw, db;
+    if (nw) dw = at::empty(w_sizes, plain(gy).dtype(w_type));
+    if (nb) db = at::empty({n}, plain(gy).dtype((at::ScalarType)types[2]));
+    if (nx) dx = at::empty(sizes, plain(gy));
+    if (s.rows == 0) {
+      if (nw) dw.zero_();
+      if (nb) db.zero_();
+    } else {
+      winoconv_linear_desc_t d = describe(s, type, act);
+      void *stream = stream_of();
+      const bool slope = act != WINOCONV_ACT_NONE;
+      // without an activation dz is gy as it lies, or a copy on 16 bytes
+      const bool copy = slope || ld_of(g) % 8 != 0 || (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) != 0;
+      at::Tensor dz = g;
+      if (((nx || nw) && copy) || nb) {
+        at::Tensor ws;
+        uint64_t bytes = 0;
+        if (nb) {
+          check_abi(winoconv_linear_backward_ws(&d, &bytes), "winoconv_linear_backward_ws");
+          ws = at::empty({(int64_t)bytes}, plain(gy).dtype(at::kByte));
+        }
+        const bool write = (nx || nw) && copy;
+        if (write) dz = at::empty({s.rows, round8(n)}, plain(gy)).narrow(1, 0, n);
+        const bool z8 = slope && pack;
+        check_abi(winoconv_linear_backward_activation(&d, g.data_ptr(), s.rows > 1 ? ld_of(g) : 0, slope && !pack ? saved[2].data_ptr() : nullptr,
+                                                      z8 ? saved[2].data_ptr() : nullptr, z8 ? saved[3].data_ptr() : nullptr, write ? dz.data_ptr() : nullptr,
+                                                      write ? round8(n) : 0, nb ? db.data_ptr() : nullptr, nb ? code_of(db.scalar_type()) : 0,
+                                                      nb ? ws.data_ptr() : nullptr, bytes, stream),
+                  "winoconv_linear_backward_activation");
+      }
+      if (nx) {
+        const at::Tensor w = operand(saved[4].scalar_type() == type ? saved[4] : saved[4].to(type));
+        d.w_stride = ld_of(w);
+        check_abi(winoconv_linear_backward_data(&d, dz.data_ptr(), ld_of(dz), w.data_ptr(), dx.data_ptr(), 0, stream), "winoconv_linear_backward_data");
+      }
+      if (nw) {
+        at::Tensor x;
+        if (pack) {      // rows on 16 bytes
+          x = at::empty({s.rows, round8(k)}, plain(gy)).narrow(1, 0, k);
+          check_abi(winoconv_e4m3_unpack(d.dtype, saved[0].data_ptr(), saved[1].data_ptr(), s.rows, (int32_t)k, x.data_ptr(), round8(k), stream), "winoconv_e4m3_unpack");
+        } else x = operand(as_rows(saved[0], k));
+        d.x_stride = ld_of(x);
+        const bool direct = w_type == at::kFloat || w_type == type;
+        TORCH_CHECK(direct, "linear: weight type");
+        check_abi(winoconv_linear_backward_weight(&d, dz.data_ptr(), ld_of(dz), x.data_ptr(), dw.data_ptr(), code_of(w_type), stream),
+                  "winoconv_linear_backward_weight");
+      }
+    }
+    out[0] = dx;
+    out[1] = dw;
+    out[2] = db;
+    return out;
+  }
+};
+
+}  // namespace
+
+at::Tensor linear_call(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, const std::optional<at::Tensor> &residual,
+                       int64_t act, bool pack) {
+  TORCH_CHECK(x.is_cuda(), "linear runs on CUDA devices only: there is no CPU path");
+  TORCH_CHECK(is16(x), "linear: x must be float16 or bfloat16, got ", x.scalar_type());
+  TORCH_CHECK(weight.dim() == 2, "linear: weight must be [out_features, in_features], got ", weight.sizes());
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == weight.size(1), "linear: x ", x.sizes(), " does not end in the weight's ", weight.size(1), " input features");
+  TORCH_CHECK(weight.size(0) > 0 && weight.size(1) > 0, "linear: weight must not be empty, got ", weight.sizes());
+  TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "linear: weight must be of x's type or float32, got ", weight.scalar_type());
+  TORCH_CHECK(weight.device() == x.device(), "linear: weight is on ", weight.device(), ", x on ", x.device());
+  if (bias) {
+    TORCH_CHECK(bias->dim() == 1 && bias->size(0) == weight.size(0), "linear: bias must be [", weight.size(0), "], got ", bias->sizes());
+    TORCH_CHECK(bias->scalar_type() == x.scalar_type() || bias->scalar_type() == at::kFloat, "linear: bias must be of x's type or float32, got ", bias->scalar_type());
+    TORCH_CHECK(bias->device() == x.device(), "linear: bias is on ", bias->device(), ", x on ", x.device());
+  }
+  if (residual) {
+    std::vector<int64_t> want(x.sizes().begin(), x.sizes().end());
+    want.back() = weight.size(0);
+    TORCH_CHECK(residual->sizes() == at::IntArrayRef(want), "linear: residual must have the output's shape ", at::IntArrayRef(want), ", got ", residual->sizes());
+    TORCH_CHECK(residual->scalar_type() == x.scalar_type(), "linear: residual must be of x's type, got ", residual->scalar_type());
+    TORCH_CHECK(residual->device() == x.device(), "linear: residual is on ", residual->device(), ", x on ", x.device());
+  }
+  TORCH_CHECK(act >= WINOCONV_ACT_NONE && act <= WINOCONV_ACT_SILU, "linear: bad activation");
+  c10::cuda::CUDAGuard guard(x.device());
+  if (at::GradMode::is_enabled() &&
+      (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) || (residual && residual->requires_grad())))
+    return LinearFn::apply(x, weight, bias, residual, act, pack);
+  at::AutoDispatchBelowADInplaceOrView no_graph;
+  return forward(x, weight, bias ? *bias : at::Tensor(), residual ? *residual : at::Tensor(), (int)act, false, false, false, nullptr);
+}
+
+std::tuple<at::Tensor, at::Tensor> e4m3_pack(const at::Tensor &x_in) {
+  TORCH_CHECK(x_in.is_cuda(), "checkpoint.pack runs on CUDA devices only: there is no CPU path");
+  TORCH_CHECK(is16(x_in), "checkpoint.pack: x must be float16 or bfloat16, got ", x_in.scalar_type());
+  TORCH_CHECK(x_in.dim() >= 1 && x_in.size(-1) > 0, "checkpoint.pack: x must have a last dimension that is not empty, got ", x_in.sizes());
+  at::AutoDispatchBelowADInplaceOrView no_graph;
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const int64_t cols = x_in.size(-1);
+  const at::Tensor x = with_rows(as_rows(x_in, cols));
+  std::vector<int64_t> sizes(x_in.sizes().begin(), x_in.sizes().end());
+  at::Tensor q = at::empty(sizes, plain(x).dtype(at::kFloat8_e4m3fn));
+  sizes.back() = (cols + 31) / 32;
+  at::Tensor scale = at::empty(sizes, plain(x).dtype(at::kFloat8_e8m0fnu));
+  TORCH_CHECK(cols <= 0x7fffffffLL, "checkpoint.pack: rows too long");
+  if (x.size(0) > 0)
+    check_abi(winoconv_e4m3_pack(code_of(x.scalar_type()), x.data_ptr(), x.size(0) > 1 ? row_stride(x) : 0, x.size(0), (int32_t)cols, q.data_ptr(), scale.data_ptr(), stream_of()),
+              "winoconv_e4m3_pack");
+  return {q, scale};
+}
+
+at::Tensor e4m3_unpack(const at::Tensor &q_in, const at::Tensor &scale_in, at::ScalarType type) {
+  TORCH_CHECK(q_in.is_cuda() && scale_in.device() == q_in.device(), "checkpoint.unpack runs on CUDA devices only, q and scale on the same one");
+  TORCH_CHECK(q_in.scalar_type() == at::kFloat8_e4m3fn && scale_in.scalar_type() == at::kFloat8_e8m0fnu,
+              "checkpoint.unpack: q must be float8_e4m3fn and scale float8_e8m0fnu, got ", q_in.scalar_type(), " and ", scale_in.scalar_type());
+  TORCH_CHECK(type == at::kHalf || type == at::kBFloat16, "checkpoint.unpack: dtype must be float16 or bfloat16, got ", type);
+  TORCH_CHECK(q_in.dim() >= 1 && q_in.size(-1) > 0, "checkpoint.unpack: q must have a last dimension that is not empty, got ", q_in.sizes());
+  std::vector<int64_t> sizes(q_in.sizes().begin(), q_in.sizes().end());
+  const int64_t cols = sizes.back();
+  sizes.back() = (cols + 31) / 32;
+  TORCH_CHECK(scale_in.sizes() == at::IntArrayRef(sizes), "checkpoint.unpack: scale must be ", at::IntArrayRef(sizes), " for q ", q_in.sizes(), ", got ", scale_in.sizes());
+  TORCH_CHECK(cols <= 0x7fffffffLL, "checkpoint.unpack: rows too long");
+  at::AutoDispatchBelowADInplaceOrView no_graph;
+  c10::cuda::CUDAGuard guard(q_in.device());
+  const at::Tensor q = q_in.contiguous(), scale = scale_in.contiguous();
+  at::Tensor x = at::empty(q.sizes(), plain(q).dtype(type));
+  const int64_t rows = q.numel() / cols;
+  if (rows > 0)
+    check_abi(winoconv_e4m3_unpack(code_of(type), q.data_ptr(), scale.data_ptr(), rows, (int32_t)cols, x.data_ptr(), 0, stream_of()), "winoconv_e4m3_unpack");
+  return x;
+}

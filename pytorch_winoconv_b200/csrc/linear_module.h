@@ -1,0 +1,19 @@
+// Native forward and backward of the fully connected layers (linear.py) and the packing of activations (checkpoint.py): layout
+// copies, allocation, launches and the autograd node without a trip through Python per call.
+#pragma once
+
+#include <cstdint>
+#include <optional>
+#include <tuple>
+
+#include <torch/extension.h>
+
+// y = act(x weight^T + bias) + residual in x's type (f16 or bf16); act: winoconv_act_t.  weight and bias are of that type or f32
+// (the weight is then rounded once, the bias added as it is).  pack: what the backward pass needs of x and of the
+// pre-activation is kept in eight bits.
+at::Tensor linear_call(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, const std::optional<at::Tensor> &residual,
+                       int64_t act, bool pack);
+
+// (e4m3 values of x's shape, scales [..., ceil(C / 32)] as e8m0) of a tensor's rows, and the values they stand for.
+std::tuple<at::Tensor, at::Tensor> e4m3_pack(const at::Tensor &x);
+at::Tensor e4m3_unpack(const at::Tensor &q, const at::Tensor &scale, at::ScalarType type);

@@ -11,6 +11,7 @@
 
 #include "wino_common.cuh"
 #include "wino_launch.h"
+#include "wino_linear.h"
 
 namespace wino {
 namespace {
@@ -849,6 +850,193 @@ int winoconv_backward_weight(const winoconv_desc_t *desc, const void *x, const v
   return WINOCONV_OK;
 }
 
+// ---- fully connected layers and eight-bit activations ------------------------------------------------------------------
+static bool is16(int dtype) { return dtype == WINOCONV_F16 || dtype == WINOCONV_BF16; }
+
+static int check_element(const void *p, unsigned bytes, const char *name) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0 ? WINOCONV_OK : fail(WINOCONV_ERR_INVALID_ARGUMENT, std::string(name) + " is not aligned to its elements");
+}
+
+// The checks that every entry of a layer makes.  The kernels count rows, columns and tiles in 32 bits.
+static int check_linear(const winoconv_linear_desc_t *d) {
+  if (!d) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null descriptor");
+  if (!is16(d->dtype)) return fail(WINOCONV_ERR_UNSUPPORTED, "fully connected layers run on f16 or bf16 operands");
+  if (d->activation < WINOCONV_ACT_NONE || d->activation > WINOCONV_ACT_SILU) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "bad activation");
+  if (d->rows <= 0 || d->in_features <= 0 || d->out_features <= 0) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  const int64_t most = 0x7fffffffLL - 1024;
+  if (d->rows > most || d->in_features > most || d->out_features > most ||
+      ((d->rows + 127) / 128) * (((int64_t)std::max(d->in_features, d->out_features) + 127) / 128) > most / 8 ||
+      (((int64_t)d->in_features + 127) / 128) * (((int64_t)d->out_features + 127) / 128) > most / 8)
+    return fail(WINOCONV_ERR_UNSUPPORTED, "matrix too large");
+  if ((d->x_stride && d->x_stride < d->in_features) || (d->w_stride && d->w_stride < d->in_features) || (d->residual_stride && d->residual_stride < d->out_features) ||
+      (d->y_stride && d->y_stride < d->out_features) || (d->z_stride && d->z_stride < d->out_features))
+    return fail(WINOCONV_ERR_INVALID_ARGUMENT, "row stride shorter than a row");
+  return WINOCONV_OK;
+}
+// A matrix that TMA reads.
+static int check_operand(const void *p, int64_t stride, int64_t cols, const char *name) {
+  if (!p) return fail(WINOCONV_ERR_INVALID_ARGUMENT, std::string("null ") + name);
+  if (!aligned16(p)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, std::string(name) + " must start on 16 bytes");
+  if (stride < cols) return fail(WINOCONV_ERR_INVALID_ARGUMENT, std::string(name) + ": row stride shorter than a row");
+  if (stride % 8 != 0) return fail(WINOCONV_ERR_INVALID_ARGUMENT, std::string(name) + ": the row stride must be a multiple of 8 (winoconv_pad_rows copies others)");
+  if (stride > (1LL << 36)) return fail(WINOCONV_ERR_UNSUPPORTED, std::string(name) + ": row stride too large");
+  return WINOCONV_OK;
+}
+static int64_t or_dense(int64_t stride, int64_t cols) { return stride ? stride : cols; }
+
+static int run_linear(const LinearProblem &p, void *stream, const char *what) {
+  const int st = winoconv_device_check();
+  if (st != WINOCONV_OK) return st;
+  const char *detail = "";
+  const cudaError_t e = launch_linear(p, linear_plan(p), (cudaStream_t)stream, &detail);
+  if (e != cudaSuccess) cudaGetLastError();      // reported here: the caller's next check of its own is not to find it
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, what, detail);
+}
+
+int winoconv_linear_forward(const winoconv_linear_desc_t *desc, const void *x, const void *w, const void *bias, const void *residual, void *y, void *z,
+                            void *z8, void *z8_scale, void *stream) {
+  int st = check_linear(desc);
+  if (st != WINOCONV_OK) return st;
+  if ((st = check_operand(x, or_dense(desc->x_stride, desc->in_features), desc->in_features, "x")) != WINOCONV_OK) return st;
+  if ((st = check_operand(w, or_dense(desc->w_stride, desc->in_features), desc->in_features, "w")) != WINOCONV_OK) return st;
+  if (!y) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null y");
+  if (!z8 != !z8_scale) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "z8 and z8_scale go together");
+  if (z8 && (reinterpret_cast<uintptr_t>(z8) & 15u)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "z8 must start on 16 bytes");
+  if ((st = check_element(bias, desc->bias_f32 ? 4 : 2, "bias")) != WINOCONV_OK || (st = check_element(residual, 2, "residual")) != WINOCONV_OK ||
+      (st = check_element(y, 2, "y")) != WINOCONV_OK || (st = check_element(z, 2, "z")) != WINOCONV_OK)
+    return st;
+  LinearProblem p = {};
+  p.dtype = desc->dtype;
+  p.rows = (int)desc->rows; p.cols = desc->out_features; p.red = desc->in_features;
+  p.r = {x, or_dense(desc->x_stride, desc->in_features), 0};
+  p.c = {w, or_dense(desc->w_stride, desc->in_features), 0};
+  p.layer = 1; p.act = desc->activation; p.bias_f32 = desc->bias_f32;
+  p.bias = bias; p.residual = residual; p.y = y; p.z = z; p.z8 = (uint8_t *)z8; p.z8_scale = (uint8_t *)z8_scale;
+  p.residual_stride = or_dense(desc->residual_stride, desc->out_features);
+  p.y_stride = or_dense(desc->y_stride, desc->out_features);
+  p.z_stride = or_dense(desc->z_stride, desc->out_features);
+  return run_linear(p, stream, "linear forward launch");
+}
+
+int winoconv_linear_backward_ws(const winoconv_linear_desc_t *desc, uint64_t *bytes) {
+  if (!bytes) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null bytes");
+  int st = check_linear(desc);
+  if (st != WINOCONV_OK) return st;
+  *bytes = (uint64_t)act_grad_chunks(desc->rows, desc->out_features) * desc->out_features * 4;
+  return WINOCONV_OK;
+}
+
+int winoconv_linear_backward_activation(const winoconv_linear_desc_t *desc, const void *gy, int64_t gy_stride, const void *z, const void *z8,
+                                        const void *z8_scale, void *dz, int64_t dz_stride, void *dbias, int dbias_dtype, void *ws, size_t ws_bytes,
+                                        void *stream) {
+  int st = check_linear(desc);
+  if (st != WINOCONV_OK) return st;
+  if (!gy) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null gy");
+  if (!dz && !dbias) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "neither dz nor dbias asked for");
+  if (!z8 != !z8_scale) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "z8 and z8_scale go together");
+  if (desc->activation != WINOCONV_ACT_NONE && !z == !z8) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "the slope of an activation needs z or z8, and not both");
+  const int64_t n = desc->out_features;
+  if (or_dense(gy_stride, n) < n || or_dense(dz_stride, n) < n) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "row stride shorter than a row");
+  if (dbias && (dbias_dtype < WINOCONV_F32 || dbias_dtype > WINOCONV_BF16)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "bad dbias_dtype");
+  if ((st = check_element(gy, 2, "gy")) != WINOCONV_OK || (st = check_element(z, 2, "z")) != WINOCONV_OK || (st = check_element(dz, 2, "dz")) != WINOCONV_OK ||
+      (st = check_element(dbias, dbias_dtype == WINOCONV_F32 ? 4 : 2, "dbias")) != WINOCONV_OK)
+    return st;
+  if (dbias) {
+    const uint64_t need = (uint64_t)act_grad_chunks(desc->rows, desc->out_features) * desc->out_features * 4;
+    if (!ws) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null ws");
+    if (!aligned16(ws)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "ws must start on 16 bytes");
+    if (ws_bytes < need) return fail(WINOCONV_ERR_WORKSPACE, "bias-gradient scratch holds " + std::to_string(ws_bytes) + " bytes; needs " + std::to_string(need));
+  }
+  if ((st = winoconv_device_check()) != WINOCONV_OK) return st;
+  ActGrad a = {};
+  a.dtype = desc->dtype; a.act = desc->activation; a.rows = desc->rows; a.cols = desc->out_features;
+  const bool act = desc->activation != WINOCONV_ACT_NONE;
+  a.gy = gy; a.z = act ? z : nullptr; a.z8 = act ? (const uint8_t *)z8 : nullptr; a.z8_scale = (const uint8_t *)z8_scale;
+  a.dz = dz; a.dbias = dbias; a.dbias_dtype = dbias_dtype; a.ws = (float *)ws;
+  a.gy_stride = or_dense(gy_stride, n); a.z_stride = or_dense(desc->z_stride, n); a.dz_stride = or_dense(dz_stride, n);
+  const cudaError_t e = launch_act_grad(a, (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "activation gradient launch");
+}
+
+int winoconv_linear_backward_data(const winoconv_linear_desc_t *desc, const void *dz, int64_t dz_stride, const void *w, void *dx, int64_t dx_stride,
+                                  void *stream) {
+  int st = check_linear(desc);
+  if (st != WINOCONV_OK) return st;
+  if ((st = check_operand(dz, or_dense(dz_stride, desc->out_features), desc->out_features, "dz")) != WINOCONV_OK) return st;
+  if ((st = check_operand(w, or_dense(desc->w_stride, desc->in_features), desc->in_features, "w")) != WINOCONV_OK) return st;
+  if (!dx) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null dx");
+  if (or_dense(dx_stride, desc->in_features) < desc->in_features) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "row stride shorter than a row");
+  if ((st = check_element(dx, 2, "dx")) != WINOCONV_OK) return st;
+  LinearProblem p = {};
+  p.dtype = desc->dtype;
+  p.rows = (int)desc->rows; p.cols = desc->in_features; p.red = desc->out_features;
+  p.r = {dz, or_dense(dz_stride, desc->out_features), 0};
+  p.c = {w, or_dense(desc->w_stride, desc->in_features), 1};
+  p.y = dx;
+  p.y_stride = or_dense(dx_stride, desc->in_features);
+  return run_linear(p, stream, "linear data gradient launch");
+}
+
+int winoconv_linear_backward_weight(const winoconv_linear_desc_t *desc, const void *dz, int64_t dz_stride, const void *x, void *dw, int dw_dtype,
+                                    void *stream) {
+  int st = check_linear(desc);
+  if (st != WINOCONV_OK) return st;
+  if ((st = check_operand(dz, or_dense(dz_stride, desc->out_features), desc->out_features, "dz")) != WINOCONV_OK) return st;
+  if ((st = check_operand(x, or_dense(desc->x_stride, desc->in_features), desc->in_features, "x")) != WINOCONV_OK) return st;
+  if (!dw) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null dw");
+  if (dw_dtype != WINOCONV_F32 && dw_dtype != desc->dtype) return fail(WINOCONV_ERR_UNSUPPORTED, "dw_dtype must be F32 or the layer's dtype");
+  if ((st = check_element(dw, dw_dtype == WINOCONV_F32 ? 4 : 2, "dw")) != WINOCONV_OK) return st;
+  LinearProblem p = {};
+  p.dtype = desc->dtype;
+  p.rows = desc->out_features; p.cols = desc->in_features; p.red = (int)desc->rows;
+  p.r = {dz, or_dense(dz_stride, desc->out_features), 1};
+  p.c = {x, or_dense(desc->x_stride, desc->in_features), 1};
+  p.y = dw; p.out_f32 = dw_dtype == WINOCONV_F32;
+  p.y_stride = desc->in_features;
+  return run_linear(p, stream, "linear weight gradient launch");
+}
+
+static int check_rows(int64_t rows, int64_t cols, int64_t stride) {
+  if (rows <= 0 || cols <= 0) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  if (or_dense(stride, cols) < cols) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "row stride shorter than a row");
+  if (cols > 0x7fffffffLL - 1024 || rows > (1LL << 40) / cols) return fail(WINOCONV_ERR_UNSUPPORTED, "matrix too large");
+  return WINOCONV_OK;
+}
+
+int winoconv_pad_rows(const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int32_t cols, void *stream) {
+  if (!x || !y) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null tensor");
+  int st = check_rows(rows, cols, x_stride);
+  if (st != WINOCONV_OK) return st;
+  if (y_stride < cols || y_stride % 8 != 0 || !aligned16(y)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "y starts on 16 bytes with a row stride that is a multiple of 8 and holds a row");
+  if (y_stride > 0x7fffffffLL - 1024) return fail(WINOCONV_ERR_UNSUPPORTED, "matrix too large");
+  if ((st = check_element(x, 2, "x")) != WINOCONV_OK) return st;
+  if ((st = winoconv_device_check()) != WINOCONV_OK) return st;
+  const cudaError_t e = launch_pad_rows(x, or_dense(x_stride, cols), y, y_stride, rows, cols, (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "row copy launch");
+}
+
+static int check_e4m3(int dtype, const void *x, int64_t x_stride, int64_t rows, int32_t cols, const void *q, const void *scale) {
+  if (!x || !q || !scale) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null tensor");
+  if (!is16(dtype)) return fail(WINOCONV_ERR_UNSUPPORTED, "eight-bit activations come from f16 or bf16 values");
+  int st = check_element(x, 2, "x");
+  if (st == WINOCONV_OK) st = check_rows(rows, cols, x_stride);
+  return st != WINOCONV_OK ? st : winoconv_device_check();
+}
+
+int winoconv_e4m3_pack(int dtype, const void *x, int64_t x_stride, int64_t rows, int32_t cols, void *q, void *scale, void *stream) {
+  const int st = check_e4m3(dtype, x, x_stride, rows, cols, q, scale);
+  if (st != WINOCONV_OK) return st;
+  const cudaError_t e = launch_e4m3_pack(dtype, x, or_dense(x_stride, cols), rows, cols, (uint8_t *)q, (uint8_t *)scale, (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "e4m3 pack launch");
+}
+
+int winoconv_e4m3_unpack(int dtype, const void *q, const void *scale, int64_t rows, int32_t cols, void *x, int64_t x_stride, void *stream) {
+  const int st = check_e4m3(dtype, x, x_stride, rows, cols, q, scale);
+  if (st != WINOCONV_OK) return st;
+  const cudaError_t e = launch_e4m3_unpack(dtype, (const uint8_t *)q, (const uint8_t *)scale, rows, cols, x, or_dense(x_stride, cols), (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "e4m3 unpack launch");
+}
+
 int winoconv_gemm_batched(int dtype, int product_dtype, int gemm_engine, int positions, int64_t tiles, int c_pad,
                           int k_out, const void *v, const void *u, void *m, void *stream) {
   if (!v || !u || !m) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null operand");
@@ -938,13 +1126,14 @@ int winoconv_read_device_error(void *stream, uint32_t *code) {
   if (!code) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null code");
   unsigned int host = 0, host2 = 0;
   cudaError_t e = read_and_clear_device_error((cudaStream_t)stream, &host);
-  unsigned int host3 = 0, host4 = 0, host5 = 0;
+  unsigned int host3 = 0, host4 = 0, host5 = 0, host6 = 0;
   if (e == cudaSuccess) e = read_and_clear_fused_error((cudaStream_t)stream, &host2);
   if (e == cudaSuccess) e = read_and_clear_row_error((cudaStream_t)stream, &host3);
   if (e == cudaSuccess) e = read_and_clear_direct_error((cudaStream_t)stream, &host4);
   if (e == cudaSuccess) e = read_and_clear_wgrad_error((cudaStream_t)stream, &host5);
+  if (e == cudaSuccess) e = read_and_clear_linear_error((cudaStream_t)stream, &host6);
   if (e != cudaSuccess) return cuda_fail(e, "reading the device error word");
-  if (host == 0) host = host2 ? host2 : host3 ? host3 : host4 ? host4 : host5;
+  if (host == 0) host = host2 ? host2 : host3 ? host3 : host4 ? host4 : host5 ? host5 : host6;
   *code = host;
   if (host != 0) return fail(WINOCONV_ERR_TIMEOUT, "a bounded device wait gave up, code 0x" + [&] { char b[16]; snprintf(b, sizeof b, "%x", host); return std::string(b); }());
   return WINOCONV_OK;

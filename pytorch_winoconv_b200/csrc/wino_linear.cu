@@ -1,0 +1,394 @@
+// Matrix products of the fully connected layers on the tensor cores (sm_100a), 16-bit operands, fp32 accumulate:
+//
+//     out[row][col] = sum over i of R[row, i] C[col, i]
+//
+//     forward          R = x  [M][K],  C = W [N][K]       z = out + bias,  y = act(z) + residual
+//     data gradient    R = dz [M][N],  C = W read down its columns        dx
+//     weight gradient  R = dz and C = x, both read down their columns     dW
+//
+// "Down its columns" is an MN-major operand of the MMA: TMA brings [reduction][64 rows] boxes as they lie, nothing is transposed
+// or copied.
+//
+// Cluster kernel: a tile of up to 256 rows x 128 columns by a cluster of CTAs that share its reduction.  The 128 columns (output
+// features) are the M side of the MMA and the rows its N side, so one row costs no more than 16 and the weights, which are what
+// has to be read when rows are few, stream through a ring of TMA stages; the parts of a tile are added up over distributed shared
+// memory, in the same order in every CTA: no scratch, no atomics, the same bits every time.  Two CTAs of an SM keep the memory
+// busy while a third party's sums travel.
+//
+// Roles: warp 0 TMA, warp 1 MMA issue; then all eight warps move the accumulator to shared memory and add up and store their share
+// of the rows.  Every mbarrier wait is bounded and reports through the error word.
+#include <algorithm>
+#include <mutex>
+#include <set>
+#include <utility>
+
+#include "wino_e4m3.cuh"
+#include "wino_launch.h"
+#include "wino_linear.h"
+
+namespace wino {
+
+__device__ unsigned int g_linear_error = 0;
+
+namespace linear {
+
+using namespace sm100;
+
+constexpr int BK = 64;                 // reduction step of a stage: 64 values of 16 bits, one row of the 128-byte swizzle
+constexpr int BC = 128;                // columns of a CTA
+constexpr int C_BYTES = BC * BK * 2;   // of a stage
+constexpr int BAR_BYTES = 256;
+constexpr int SMS = 148;               // of a B200: what plans are made for
+
+enum ErrCode : unsigned { ERR_EMPTY = 0x601, ERR_FULL = 0x602, ERR_DONE = 0x603, ERR_ACC_EMPTY = 0x604, ERR_ACC_FULL = 0x605 };
+
+// What the epilogues need of a problem.
+struct Out {
+  int rows, cols, act, layer, bias_f32, out_f32, wide;      // wide: rows of y, z and residual take vectors
+  const void *bias, *residual;
+  void *y, *z;
+  uint8_t *z8, *z8_scale;
+  long long residual_stride, y_stride, z_stride;
+};
+
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+// `n` rows from `row` on, reduction from `k` on: one box, or a box per 64 rows where the rows lie contiguous.
+__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap *map, uint32_t bar, int mn, int row, int n, int k) {
+  if (!mn) tma_load_2d(dst, map, bar, k, row);
+  else
+    for (int j = 0; j < n; j += 64) tma_load_2d(dst + (uint32_t)j * 128u, map, bar, row + j, k);
+}
+// Low descriptor word of an operand tile and the step between its 16-value slices (16-byte units).  MN-major: blocks of 64 rows
+// 8 KB apart, groups of eight reduction steps 1 KB apart; K-major: groups of eight rows 1 KB apart.
+__device__ __forceinline__ uint32_t operand_lo(uint32_t saddr, int mn) { return desc_lo(saddr, mn ? 8192u : 16u); }
+__device__ __forceinline__ uint32_t operand_step(int mn) { return mn ? 128u : 2u; }
+
+// Four neighbouring columns of a row, summed: bias, activation, residual, and what is kept of z.
+template <typename T>
+__device__ __forceinline__ void finish4(const Out &o, int row, int col, float (&v)[4]) {
+  const bool any = col < o.cols;
+  if (o.layer) {
+    if (o.bias) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < o.cols) v[j] += o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[col + j] : Elem<T>::load((const T *)o.bias + col + j);
+    }
+    if (o.z8) {      // (columns beyond the last are zero: no part in a block's scale)
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = fmaxf(top, e4m3::finite_magnitude(v[j]));
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const uint32_t byte = e4m3::scale_byte(top);
+      const float inv = e4m3::inverse_scale(byte);
+      const uint32_t q = e4m3::pack2(v[0], v[1], inv) | (e4m3::pack2(v[2], v[3], inv) << 16);
+      if (any) {
+        uint8_t *dst = o.z8 + (long long)row * o.cols + col;
+        if ((o.cols & 3) == 0) *reinterpret_cast<uint32_t *>(dst) = q;
+        else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (col + j < o.cols) dst[j] = (uint8_t)(q >> (8 * j));
+        }
+        if ((col & (e4m3::BLOCK - 1)) == 0) o.z8_scale[(long long)row * ((o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK) + col / e4m3::BLOCK] = (uint8_t)byte;
+      }
+    }
+    if (!any) return;
+    if (o.z) {
+      T *dst = (T *)o.z + row * o.z_stride + col;
+      if (o.wide) VecIO<T, 4>::store(dst, v);
+      else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < o.cols) Elem<T>::store(dst + j, v[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = act::apply(v[j], o.act);
+    if (o.residual) {
+      const T *src = (const T *)o.residual + row * o.residual_stride + col;
+      float r[4] = {0.f, 0.f, 0.f, 0.f};
+      if (o.wide) VecIO<T, 4>::load(src, r);
+      else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (col + j < o.cols) r[j] = Elem<T>::load(src + j);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += r[j];
+    }
+  }
+  if (!any) return;
+  if (o.out_f32) {
+    float *dst = (float *)o.y + row * o.y_stride + col;
+    if (o.wide) VecIO<float, 4>::store(dst, v);
+    else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < o.cols) dst[j] = v[j];
+    }
+  } else {
+    T *dst = (T *)o.y + row * o.y_stride + col;
+    if (o.wide) VecIO<T, 4>::store(dst, v);
+    else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col + j < o.cols) Elem<T>::store(dst + j, v[j]);
+    }
+  }
+}
+
+struct ClusterArgs {
+  int n_steps, n_rt, tile_rows, stages, r_mn, c_mn;
+  uint32_t idesc;
+};
+
+constexpr int CLUSTER_THREADS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(CLUSTER_THREADS, 2)
+    cluster_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Out o,
+                   const __grid_constant__ ClusterArgs g, int split) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *base_ptr = smem_raw + (base - raw);
+  const uint32_t stage_bytes = (uint32_t)(C_BYTES + g.tile_rows * BK * 2);
+  // the barriers lie behind the ring or the sums, whichever is longer
+  const uint32_t ring = max((uint32_t)g.stages * stage_bytes, (uint32_t)(g.tile_rows * BC * 4));
+  const uint32_t bars = base + ring;      // full[8] empty[8] done
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 64u + 8u * i; };
+  const uint32_t done = bars + 128u, tmem_slot = bars + 196u;
+  volatile unsigned *abort_word = reinterpret_cast<volatile unsigned *>(base_ptr + ring + 192);
+  unsigned *err = &g_linear_error;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  const uint32_t part = split > 1 ? cluster_ctarank() : 0u;
+  const int tile = (int)blockIdx.x / split, ct = tile / g.n_rt, rt = tile - ct * g.n_rt;      // CTAs in flight share columns: the weights are read once
+  const int row0 = rt * g.tile_rows, col0 = ct * BC;
+  const int k0 = (int)((long long)g.n_steps * part / split), k1 = (int)((long long)g.n_steps * (part + 1) / split);
+  uint32_t tmem_cols = 32;
+  while (tmem_cols < (uint32_t)g.tile_rows) tmem_cols *= 2;
+
+  if (warp == 1 && lane == 0) { prefetch_map(&map_r); prefetch_map(&map_c); }
+  if (warp == 0) {
+    if (lane < 8) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
+    else if (lane == 8) mbar_init(done, 1);
+    else if (lane == 9) *abort_word = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 2) tmem_alloc<false>(tmem_slot, tmem_cols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  if (warp == 0) {
+    int s = 0;
+    uint32_t ph = 1;
+    for (int k = k0; k < k1; ++k) {
+      if (!mbar_wait_warp(empty(s), ph, abort_word, err, ERR_EMPTY)) break;
+      if (lane == 0) {
+        mbar_expect_tx(full(s), stage_bytes);
+        const uint32_t dst = base + (uint32_t)s * stage_bytes;
+        load_operand(dst, &map_c, full(s), g.c_mn, col0, BC, k * BK);
+        load_operand(dst + C_BYTES, &map_r, full(s), g.r_mn, row0, g.tile_rows, k * BK);
+      }
+      if (++s == g.stages) { s = 0; ph ^= 1u; }
+    }
+    if (*abort_word != 0u) {   // loads in flight must land before the shared memory goes away
+      const long long start = clock64();
+      while (clock64() - start < 2000000LL) { }
+    }
+  } else if (warp == 1) {
+    int s = 0;
+    uint32_t ph = 0;
+    bool alive = true;
+    for (int k = k0; k < k1; ++k) {
+      if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
+      tc_fence_after();
+      const uint32_t st = base + (uint32_t)s * stage_bytes;
+      const uint32_t a = operand_lo(st, g.c_mn), b = operand_lo(st + C_BYTES, g.r_mn), hi = desc_hi(1024, 2);
+      if (elect_one()) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          umma<false, false>(tmem, a + (uint32_t)j * operand_step(g.c_mn), hi, b + (uint32_t)j * operand_step(g.r_mn), hi, g.idesc, (k > k0 || j > 0) ? 1u : 0u);
+        umma_commit<false>(empty(s), 0);
+      }
+      __syncwarp();
+      if (++s == g.stages) { s = 0; ph ^= 1u; }
+    }
+    if (alive && elect_one()) umma_commit<false>(done, 0);
+  }
+  __syncwarp();
+  // sums to shared memory: [row][128 columns]
+  const bool ok = mbar_wait_warp(done, 0, abort_word, err, ERR_DONE);
+  float *sums = reinterpret_cast<float *>(base_ptr);
+  if (ok && *abort_word == 0u) {
+    tc_fence_after();
+    const int q = warp & 3;
+    for (int c = (warp >> 2) * 32; c < g.tile_rows; c += 64) {
+      uint32_t v[32];
+      tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
+      tmem_wait_ld_x32(v);
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (c + j < g.tile_rows) sums[(c + j) * BC + q * 32 + lane] = __uint_as_float(v[j]);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (split > 1) cluster_sync_all();
+  if (*abort_word == 0u) {
+    const int n = min(g.tile_rows, o.rows - row0);
+    for (int j = (int)part + warp * split; j < n; j += 8 * split) {
+      float v[4];
+      const uint32_t src = base + (uint32_t)((j * BC + lane * 4) * 4);
+      if (split == 1) {
+        const float4 u = *reinterpret_cast<const float4 *>(sums + j * BC + lane * 4);
+        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+      } else {
+        auto add_parts = [&](auto n_parts) {      // all parts' values in flight at once, added in the same order by every CTA
+          constexpr int S = decltype(n_parts)::value;
+          float4 u[S];
+#pragma unroll
+          for (int i = 0; i < S; ++i) u[i] = ld_cluster_f4(map_to_rank(src, (uint32_t)i));
+          v[0] = u[0].x; v[1] = u[0].y; v[2] = u[0].z; v[3] = u[0].w;
+#pragma unroll
+          for (int i = 1; i < S; ++i) { v[0] += u[i].x; v[1] += u[i].y; v[2] += u[i].z; v[3] += u[i].w; }
+        };
+        if (split == 2) add_parts(std::integral_constant<int, 2>());
+        else if (split == 4) add_parts(std::integral_constant<int, 4>());
+        else add_parts(std::integral_constant<int, 8>());
+      }
+      finish4<T>(o, row0 + j, col0 + lane * 4, v);
+    }
+  }
+  __syncwarp();
+  if (split > 1) cluster_sync_all();      // no CTA leaves while another reads its shared memory
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_free<false>(tmem, tmem_cols);
+  }
+}
+
+// Boxes of 64 x `rows` (K-major) or 64 rows x 64 reduction steps (MN-major), zeros beyond the operand's ends.
+bool operand_map(CUtensorMap *m, EncodeTiledFn enc, int dtype, const MatOperand &p, int rows, int red, int box_rows) {
+  cuuint64_t dims[2] = {(cuuint64_t)(p.mn ? rows : red), (cuuint64_t)(p.mn ? red : rows)}, st[1] = {(cuuint64_t)p.stride * 2};
+  cuuint32_t box[2] = {64u, p.mn ? 64u : (cuuint32_t)box_rows}, es[2] = {1u, 1u};
+  return enc(m, map_dtype(dtype), 2, const_cast<void *>(p.ptr), dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint32_t instruction(int dtype, int a_mn, int b_mn, int m, int n) {
+  const uint32_t fmt = dtype == WINOCONV_F16 ? 0u : 1u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+bool multiple(const void *p, long long stride, int el, int bytes) {
+  return (reinterpret_cast<uintptr_t>(p) % (uintptr_t)bytes) == 0 && stride * el % bytes == 0;
+}
+
+Out out_of(const LinearProblem &p, int width) {      // width: columns of a vector access
+  Out o;
+  o.rows = p.rows; o.cols = p.cols; o.act = p.act; o.layer = p.layer; o.bias_f32 = p.bias_f32; o.out_f32 = p.out_f32;
+  o.bias = p.bias; o.residual = p.residual; o.y = p.y; o.z = p.z; o.z8 = p.z8; o.z8_scale = p.z8_scale;
+  o.residual_stride = p.residual_stride; o.y_stride = p.y_stride; o.z_stride = p.z_stride;
+  const int el = p.out_f32 ? 4 : 2;
+  o.wide = p.cols % width == 0 && multiple(p.y, p.y_stride, el, std::min(16, el * width)) && (!p.residual || multiple(p.residual, p.residual_stride, 2, 2 * width)) &&
+           (!p.z || multiple(p.z, p.z_stride, 2, 2 * width));
+  return o;
+}
+
+// All of an SM's shared memory for a kernel, asked for once on each device.
+cudaError_t allow_smem(const void *kern) {
+  static std::mutex mu;
+  static std::set<std::pair<const void *, int>> done;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (done.count({kern, dev})) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess) done.insert({kern, dev});
+  return e;
+}
+
+int cluster_smem(const LinearPlan &plan) {
+  return 1024 + std::max(plan.stages * (C_BYTES + plan.tile_rows * BK * 2), plan.tile_rows * BC * 4) + BAR_BYTES;
+}
+
+template <typename T>
+cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  CUtensorMap mr, mc;
+  if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, plan.tile_rows) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, BC)) {
+    *detail = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  auto kern = cluster_kernel<T>;
+  cudaError_t e = allow_smem((const void *)kern);
+  if (e != cudaSuccess) return e;
+  ClusterArgs g;
+  g.n_steps = (p.red + BK - 1) / BK;
+  g.n_rt = (p.rows + plan.tile_rows - 1) / plan.tile_rows;
+  g.tile_rows = plan.tile_rows; g.stages = plan.stages; g.r_mn = p.r.mn; g.c_mn = p.c.mn;
+  g.idesc = instruction(p.dtype, p.c.mn, p.r.mn, 128, plan.tile_rows);
+  const int n_ct = (p.cols + BC - 1) / BC;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(g.n_rt * n_ct * plan.split)); cfg.blockDim = dim3(CLUSTER_THREADS);
+  cfg.dynamicSmemBytes = (size_t)cluster_smem(plan); cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)plan.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = plan.split > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 4), g, plan.split);
+}
+
+}  // namespace linear
+
+using namespace linear;
+
+// Tile and cluster of a problem: rows to a tile as many as there are, up to 128; then as many CTAs to a tile's reduction as
+// bring the grid nearest to two on every SM from below.
+LinearPlan linear_plan(const LinearProblem &p) {
+  LinearPlan plan = {};
+  const int unit = p.r.mn ? 64 : 16;
+  plan.tile_rows = std::min(128, (p.rows + unit - 1) / unit * unit);
+  const long long tiles = (long long)((p.rows + plan.tile_rows - 1) / plan.tile_rows) * ((p.cols + BC - 1) / BC);
+  const int n_steps = (p.red + BK - 1) / BK;
+  plan.split = 1;
+  while (plan.split < 8 && tiles * plan.split * 2 <= 2LL * SMS && plan.split * 2 <= n_steps) plan.split *= 2;
+  const int budget = 113 * 1024 - 1024 - 1024 - BAR_BYTES;      // of an SM's 228 KB with 1 KB of the system's for each CTA
+  plan.stages = std::min(8, budget / (C_BYTES + plan.tile_rows * BK * 2));
+  return plan;
+}
+
+cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
+  *detail = "";
+  EncodeTiledFn enc = encode_tiled_fn();
+  if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
+  return p.dtype == WINOCONV_F16 ? launch_cluster<__half>(p, plan, enc, s, detail) : launch_cluster<__nv_bfloat16>(p, plan, enc, s, detail);
+}
+
+cudaError_t read_and_clear_linear_error(cudaStream_t s, unsigned int *code) {
+  unsigned int host = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(&host, g_linear_error, sizeof(host), 0, cudaMemcpyDeviceToHost, s);
+  if (e == cudaSuccess) e = cudaMemcpyToSymbolAsync(g_linear_error, &zero, sizeof(zero), 0, cudaMemcpyHostToDevice, s);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+  *code = host;
+  return e;
+}
+
+}  // namespace wino

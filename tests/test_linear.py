@@ -1,0 +1,534 @@
+"""Fully connected layers (``linear``) against their formulas in 64 bits.
+
+Most inputs are small integers times powers of two: then every product and every sum of the layer is exact in fp32, and what the
+kernels return is the exact value rounded once -- equality is asked for, not closeness.  With the smooth activations the tolerance
+counts, per element, the rounding of the result (half a step: ``eps / 2`` relative) and 2^-18 of what an fp32 activation is made
+of (its exponential and division are good to a few 2^-22, the arguments of the exponential lose up to 2^-23 times their size,
+which is below 16 where the slope is not flat), and for products of a rounded gradient half a step of each of its values."""
+import ctypes
+
+import pytest
+import torch
+
+from pytorch_winoconv_b200 import capi, checkpoint, linear as lin
+
+gpu = pytest.mark.gpu
+DTYPES = [torch.float16, torch.bfloat16]
+F = torch.nn.functional
+
+
+def ints(shape, seed, span, step, dtype, device="cuda"):
+    """Integers of -span..span times step."""
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randint(-span, span + 1, shape, generator=g).double() * step).to(dtype).to(device)
+
+
+def act64(z, name):
+    return {None: lambda t: t, "relu": F.relu, "gelu": F.gelu, "gelu_tanh": lambda t: F.gelu(t, approximate="tanh"), "silu": F.silu}[name](z)
+
+
+def half_step(t, dtype):
+    """Half a step of the type at each value, and of its subnormals."""
+    info = torch.finfo(dtype)
+    return t.abs() * (info.eps / 2) + info.smallest_normal * info.eps / 2
+
+
+def make(rows, k, n, dtype, seed=0, bias=True, residual=True):
+    """Layer inputs whose sums are exact: |x| <= 2, |w| <= 1/2 in steps of 1/4 and 1/8, so sums are multiples of 2^-5 below 2^15."""
+    x = ints((rows, k), seed, 8, 0.25, dtype)
+    w = ints((n, k), seed + 1, 4, 0.125, dtype)
+    b = ints((n,), seed + 2, 8, 0.25, dtype) if bias else None
+    r = ints((rows, n), seed + 3, 8, 0.25, dtype) if residual else None
+    return x, w, b, r
+
+
+def forward64(x, w, b, r, act):
+    z = x.double() @ w.double().t()
+    if b is not None:
+        z = z + b.double()
+    y = act64(z, act)
+    return z, y if r is None else y + r.double()
+
+
+def check(got, want, act, dtype, extra=None):
+    """Equal to the exact value rounded once, or within the tolerance of a smooth activation."""
+    if act in (None, "relu") and extra is None:
+        assert torch.equal(got, want.to(dtype))
+        return
+    tol = half_step(want, dtype) + want.abs() * 2.0 ** -18 + (0 if extra is None else extra)
+    off = (got.double() - want).abs()
+    assert (off <= tol).all(), ((off - tol).max().item(), off.max().item())
+
+
+SHAPES = [(1, 64, 128), (1, 1, 1), (1, 1000, 1531), (2, 33, 7), (3, 4096, 250), (16, 72, 136), (17, 129, 131), (31, 520, 2048), (64, 2048, 129),
+          (127, 40, 64), (128, 64, 128), (129, 65, 129), (130, 777, 1000), (257, 200, 520), (1000, 136, 96), (1025, 100, 300), (513, 1024, 768)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", SHAPES)
+def test_forward_is_the_exact_value_rounded_once(rows, k, n, dtype):
+    for i, (act, bias, residual) in enumerate([(None, False, False), ("relu", True, False), (None, True, True), ("relu", False, True)]):
+        x, w, b, r = make(rows, k, n, dtype, 10 * i, bias, residual)
+        y = lin.linear(x, w, b, r, activation=act)
+        assert y.shape == (rows, n) and y.dtype == dtype
+        check(y, forward64(x, w, b, r, act)[1], act, dtype)
+    assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 128), (17, 129, 131), (300, 40, 520)])
+def test_smooth_activations(rows, k, n, act, dtype):
+    x, w, b, r = make(rows, k, n, dtype)
+    z, y = forward64(x, w, b, r, act)
+    # fp32 error of the activation (relative to z: 1 + erf cancels for negative z), then of the sum
+    check(lin.linear(x, w, b, r, activation=act), y, act, dtype, extra=(z.abs() + 1) * 2.0 ** -20)
+    y = act64(z, act)
+    check(lin.linear(x, w, b, activation=act), y, act, dtype, extra=(z.abs() + 1) * 2.0 ** -20)
+
+
+def reference_backward(x, w, gy, z, act, dtype, bits8):
+    """dz, and the gradients from what was kept."""
+    if bits8:
+        kept_x, kept_z = values8(x.double(), dtype), values8(z, dtype)
+    else:
+        kept_x, kept_z = x.double(), z.to(dtype).double()
+    kept_z.requires_grad_()
+    dz, = torch.autograd.grad(act64(kept_z, act), kept_z, gy.double())
+    return dz, kept_x
+
+
+def values8(x, dtype):
+    """The values that eight bits hold, in 64 bits: rounding to the step at each value, half to even."""
+    out = torch.empty_like(x)
+    for c in range(0, x.shape[-1], 32):
+        v = x[..., c:c + 32]
+        top = torch.where(v.abs() < float("inf"), v.abs(), torch.zeros_like(v)).nan_to_num(0.0).amax(-1, keepdim=True)
+        m, e = torch.frexp(top)
+        e = torch.where(top > 0, e - 9 + (m > 0.875).int(), torch.full_like(e, -127)).clamp_min(-127).double()
+        t = v / torch.exp2(e)
+        _, at = torch.frexp(t.abs().clamp_min(2.0 ** -6))
+        step = torch.exp2((at - 4).double())
+        q = torch.where(t.abs() < float("inf"), torch.round(t / step) * step, torch.full_like(t, float("nan")))
+        out[..., c:c + 32] = q * torch.exp2(e)
+    most = torch.finfo(dtype).max
+    return out.clamp(-most, most)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+@pytest.mark.parametrize("rows,k,n", [s for s in SHAPES if s[0] * s[1] * s[2] < 2e8])
+def test_gradients_are_exact_values_rounded_once(rows, k, n, pack, dtype):
+    """Integer gradients of 9 values: dz is exact, and so are the sums of the three products."""
+    for act in (None, "relu"):
+        x, w, b, r = make(rows, k, n, dtype, 5)
+        gy = ints((rows, n), 9, 4, 2.0 ** -6, dtype)
+        for t in (x, w, b, r):
+            t.requires_grad_()
+        y = lin.linear(x, w, b, r, activation=act, checkpoint=pack)
+        z, want = forward64(x.detach(), w.detach(), b.detach(), r.detach(), act)
+        check(y.detach(), want, act, dtype)
+        dx, dw, db, dr = torch.autograd.grad(y, (x, w, b, r), gy)
+        dz, kept = reference_backward(x.detach(), w.detach(), gy, z, act, dtype, pack)
+        assert torch.equal(dx, (dz @ w.detach().double()).to(dtype))
+        assert torch.equal(dw, (dz.t() @ kept).to(dtype))
+        assert torch.equal(db, dz.sum(0).to(dtype))
+        assert torch.equal(dr, gy)
+    assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 128), (33, 72, 130), (200, 129, 264)])
+def test_gradients_through_smooth_activations(rows, k, n, act, pack, dtype):
+    x, w, b, _ = make(rows, k, n, dtype, 7)
+    gy = ints((rows, n), 9, 4, 2.0 ** -3, dtype)
+    for t in (x, w, b):
+        t.requires_grad_()
+    y = lin.linear(x, w, b, activation=act, checkpoint=pack)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), gy)
+    wd, xd = w.detach().double(), x.detach().double()
+    z = xd @ wd.t() + b.detach().double()
+    dz, kept = reference_backward(xd, wd, gy, z, act, dtype, pack)
+    # dz: fp32 slope (at most 1.13) times gy, then half a step of the type; the sums of n and of rows such values in fp32
+    off = gy.double().abs() * 2.0 ** -18
+    tol_dz = off + half_step(dz, dtype) + off * torch.finfo(dtype).eps
+    sums = 2.0 ** -23
+    check(dx, dz @ wd, act, dtype, extra=tol_dz @ wd.abs() + (dz.abs() @ wd.abs()) * (n / 16 + 8) * sums)
+    check(dw, dz.t() @ kept, act, dtype, extra=tol_dz.t() @ kept.abs() + (dz.abs().t() @ kept.abs()) * (rows / 16 + 8) * sums)
+    check(db, dz.sum(0), act, dtype, extra=off.sum(0) + dz.abs().sum(0) * (rows / 8 + 16) * sums)
+
+
+@gpu
+@pytest.mark.parametrize("act", [None, "gelu", "silu"])
+def test_gradients_against_differences(act):
+    """The derivative of sum(gy y) along a direction of each input, by central differences of the 64-bit layer."""
+    x, w, b, r = (t.detach().requires_grad_() for t in make(20, 40, 48, torch.float16, 3))
+    gy = ints((20, 48), 4, 8, 0.125, torch.float16)
+    grads = torch.autograd.grad(lin.linear(x, w, b, r, activation=act), (x, w, b, r), gy)
+    leaves = [t.detach().double() for t in (x, w, b, r)]
+    for i, g in enumerate(grads):
+        d = torch.randn(leaves[i].shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64).cuda()
+
+        def value(h):
+            at = [t + h * d if j == i else t for j, t in enumerate(leaves)]
+            return (forward64(*at, act)[1] * gy.double()).sum().item()
+
+        slope = (value(1e-5) - value(-1e-5)) / 2e-5
+        got = (g.double() * d).sum().item()
+        # every value of g is within two half steps (dz and the result) and z's own rounding: 2^-11 each, |act''| <= 0.8 and |z| < 64
+        assert abs(got - slope) <= (g.double() * d).abs().sum().item() * 2.0 ** -9 + 1e-6 + abs(slope) * 2.0 ** -8
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_views_strides_and_types_of_the_arguments(dtype):
+    rows, k, n = 48, 72, 104
+    x, w, b, r = make(rows, k, n, dtype)
+    want = forward64(x, w, b, r, None)[1].to(dtype)
+    wide = torch.full((rows, k + 24), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 8:8 + k] = x
+    assert torch.equal(lin.linear(wide[:, 8:8 + k], w, b, r), want)                     # rows apart, read as they lie
+    wide[:, 3:3 + k] = x
+    assert torch.equal(lin.linear(wide[:, 3:3 + k], w, b, r), want)                     # not on 16 bytes: copied
+    assert torch.equal(lin.linear(x.t().contiguous().t(), w.t().contiguous().t(), b, r.t().contiguous().t()), want)
+    both = torch.stack([b, b], 1)[:, 0]
+    assert both.stride(0) == 2 and torch.equal(lin.linear(x, w, both, r), want)
+    shifted = torch.cat([torch.zeros(1, dtype=dtype, device="cuda"), b])[1:]
+    assert torch.equal(lin.linear(x, w, shifted, r), want)
+    rw = torch.full((rows, n + 5), float("nan"), dtype=dtype, device="cuda")
+    rw[:, 1:n + 1] = r
+    assert torch.equal(lin.linear(x, w, b, rw[:, 1:n + 1]), want)                       # a residual anywhere
+    assert torch.equal(lin.linear(x, w.float(), b.float(), r), want)
+    y = lin.linear(x.reshape(4, 3, 4, k), w, b, r.reshape(4, 3, 4, n))
+    assert y.shape == (4, 3, 4, n) and torch.equal(y.reshape(rows, n), want)
+    assert torch.equal(lin.linear(x[5], w, b, r[5]), want[5])                           # one row without a batch
+    one = x[:1].expand(rows, k)
+    assert torch.equal(lin.linear(one, w, b, r[:1].expand(rows, n)), want[:1].expand(rows, n))
+    turned = x.reshape(6, 8, k).transpose(0, 1)
+    assert torch.equal(lin.linear(turned, w, b), lin.linear(x, w, b).reshape(6, 8, n).transpose(0, 1))
+
+
+@gpu
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+def test_gradients_of_views_and_of_float_parameters(pack):
+    rows, k, n, dtype = 40, 36, 50, torch.bfloat16
+    x, w, b, _ = make(rows, k, n, dtype)
+    gy = ints((rows, n), 9, 4, 2.0 ** -6, dtype)
+    xd, wd, gd = x.double(), w.double(), gy.double()
+    kept = values8(xd, dtype) if pack else xd
+    base = torch.zeros(rows, k + 3, dtype=dtype, device="cuda")
+    base[:, 2:2 + k] = x
+    base.requires_grad_()
+    wf, bf = w.float().requires_grad_(), b.float().requires_grad_()
+    y = lin.linear(base[:, 2:2 + k], wf, bf, checkpoint=pack)
+    spread = torch.zeros(rows, 2 * n, dtype=dtype, device="cuda")
+    spread[:, ::2] = gy
+    dbase, dw, db = torch.autograd.grad(y, (base, wf, bf), spread[:, ::2])              # a gradient with gaps
+    assert torch.equal(dbase[:, 2:2 + k], (gd @ wd).to(dtype)) and dbase[:, :2].abs().sum() == 0
+    assert dw.dtype == torch.float32 and torch.equal(dw, (gd.t() @ kept).float())
+    assert db.dtype == torch.float32 and torch.equal(db, gd.sum(0).float())
+    # the gradient behind a sum: one value with strides of zero
+    y = lin.linear(x.requires_grad_(), w, b, checkpoint=pack)
+    dx, = torch.autograd.grad(y.sum(), x)
+    assert torch.equal(dx, wd.sum(0).expand(rows, k).to(dtype))
+    # a row used many times over
+    one = x.detach()[:1].clone().requires_grad_()
+    y = lin.linear(one.expand(rows, k), w, b, checkpoint=pack)
+    dx, = torch.autograd.grad(y, one, gy)
+    parts = (gd @ wd).to(dtype).double()
+    assert ((dx.double() - parts.sum(0)).abs() <= half_step(parts.sum(0), dtype) + parts.abs().sum(0) * 2.0 ** -23 * rows).all()
+
+
+@gpu
+def test_only_what_is_asked_for_is_kept_and_computed():
+    rows, k, n, dtype = 256, 512, 1024, torch.bfloat16
+    x, w, b, r = make(rows, k, n, dtype)
+
+    def kept(wanted, **kw):
+        leaves = {"x": x, "w": w, "b": b, "r": r}
+        for name, t in leaves.items():
+            t.requires_grad_(name in wanted)
+        size = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: size.append(t.numel() * t.element_size()) or t, lambda t: t):
+            y = lin.linear(x, w, b, r, **kw)
+        grads = torch.autograd.grad(y, [leaves[i] for i in wanted], torch.ones_like(y))
+        assert all(g.shape == leaves[i].shape for g, i in zip(grads, wanted))
+        return sum(size)
+
+    w_, x_, z_ = 2 * n * k, 2 * rows * k, 2 * rows * n
+    assert kept("x") == w_
+    assert kept("w") == x_
+    assert kept("b") == 0 and kept("r") == 0
+    assert kept("xwbr", activation="gelu") == w_ + x_ + z_
+    assert kept("r", activation="gelu") == 0
+    assert kept("xwbr", activation="gelu", checkpoint="e4m3") == w_ + (x_ + z_) // 2 + (x_ + z_) // 64
+    for t in (x, w, b, r):
+        t.requires_grad_(False)
+    assert lin.linear(x, w, b, r).grad_fn is None
+    x.requires_grad_()
+    with torch.no_grad():
+        assert lin.linear(x, w, b, r).grad_fn is None
+
+
+@gpu
+def test_no_rows():
+    x, w, b, r = (t.requires_grad_() for t in make(2, 24, 40, torch.float16))
+    y = lin.linear(x[:0], w, b, r[:0], activation="gelu", checkpoint="e4m3")
+    assert y.shape == (0, 40)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty_like(y))
+    assert dx.abs().sum() == 0 and dw.abs().sum() == 0 and db.abs().sum() == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 70, 300])
+def test_infinities_and_nan_stay_in_their_rows(rows):
+    dtype = torch.bfloat16
+    x, w, b, r = make(rows, 200, 260, dtype)
+    want = lin.linear(x, w, b, r, activation="relu")
+    bad = x.clone()
+    bad[rows // 2, 7] = float("inf")
+    bad[0, 199] = float("nan")
+    y = lin.linear(bad, w, b, r, activation="relu")
+    ok = torch.ones(rows, dtype=torch.bool)
+    ok[0] = ok[rows // 2] = False
+    assert torch.equal(y[ok.cuda()], want[ok.cuda()])
+    assert y[0].isnan().all()
+    # operands end at their last value: what lies behind them in memory takes no part
+    pool = torch.full((rows + 3, 208 + 16), float("nan"), dtype=dtype, device="cuda")
+    pool[:rows, :200] = x
+    assert torch.equal(lin.linear(pool[:rows, :200], w, b, r, activation="relu"), want)
+    gpool = torch.full((rows + 3, 264), float("nan"), dtype=dtype, device="cuda")
+    gpool[:rows, :260] = 0.5
+    leaves = [t.detach().requires_grad_() for t in (x, w)]
+    for got, g in ((gpool[:rows, :260], torch.full((rows, 260), 0.5, dtype=dtype, device="cuda")),):
+        a = torch.autograd.grad(lin.linear(*leaves), leaves, got)
+        c = torch.autograd.grad(lin.linear(*leaves), leaves, g)
+        assert all(torch.equal(i, j) for i, j in zip(a, c))
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n", [(1, 4096, 4096), (24, 2048, 8192), (300, 1000, 1531), (2048, 1024, 1024)])
+def test_the_same_bits_every_time(rows, k, n):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, w, gy = (torch.randn(*s, device="cuda", generator=g).bfloat16() for s in ((rows, k), (n, k), (rows, n)))
+    b = torch.randn(n, device="cuda", generator=g).bfloat16()
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def once():
+        y = lin.linear(x, w, b, activation="silu", checkpoint="e4m3")
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    first = once()
+    for _ in range(3):
+        assert all(torch.equal(i, j) for i, j in zip(first, once()))
+    # and close to the exact values: sums of k, n and rows products in fp32, once or twice rounded
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    y = F.silu(z)
+    err = ((first[0].double() - y).norm() / y.norm()).item()
+    assert err < 2.0 ** -8, err
+
+
+@gpu
+def test_nothing_beyond_the_outputs_is_written():
+    """Through the C ABI: an output with gaps between its rows and rows behind its last."""
+    lib = capi.lib()
+    for dtype, code in ((torch.float16, capi.F16), (torch.bfloat16, capi.BF16)):
+        for rows, k, n in ((3, 64, 130), (300, 72, 200), (257, 136, 31)):
+            x, w, b, _ = make(rows, k, n, dtype)
+            y = torch.full((rows + 2, n + 6), 7.0, dtype=dtype, device="cuda")
+            z8 = torch.full((rows + 1, n), 9, dtype=torch.uint8, device="cuda")
+            zs = torch.full((rows + 1, (n + 31) // 32), 9, dtype=torch.uint8, device="cuda")
+            d = capi.LinearDesc(rows=rows, in_features=k, out_features=n, dtype=code, activation=0, y_stride=n + 6)
+            capi.check(lib.winoconv_linear_forward(ctypes.byref(d), x.data_ptr(), w.data_ptr(), b.data_ptr(), None, y.data_ptr(), None, z8.data_ptr(), zs.data_ptr(),
+                                                   torch.cuda.current_stream().cuda_stream), "forward")
+            z, want = forward64(x, w, b, None, None)
+            assert torch.equal(y[:rows, :n], want.to(dtype))
+            assert (y[rows:] == 7).all() and (y[:, n:] == 7).all()
+            assert (z8[rows:] == 9).all() and (zs[rows:] == 9).all()
+            # sums are exact in fp32, so the eight bits are those of the exact z
+            q = z8[:rows].view(torch.float8_e4m3fn).double()
+            s = zs[:rows].view(torch.float8_e8m0fnu).float().double().repeat_interleave(32, 1)[:, :n]
+            assert torch.equal((q * s), values8(z, torch.bfloat16))
+
+
+@gpu
+def test_streams_and_graphs():
+    rows, k, n, dtype = 200, 264, 392, torch.bfloat16
+    x, w, b, r = make(rows, k, n, dtype)
+    gy = ints((rows, n), 9, 4, 2.0 ** -6, dtype)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = lin.linear(*leaves, activation="silu", checkpoint="e4m3")
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert all(torch.equal(i, j) for i, j in zip(got, want))
+    # two graphs, replayed with other values and in turn: nothing is shared between them or kept from the capture
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step()
+        graphs.append((g, out))
+    x.copy_(ints(x.shape, 77, 8, 0.25, dtype))
+    w.copy_(ints(w.shape, 78, 4, 0.125, dtype))
+    want = step()
+    for g, _ in graphs:
+        g.replay()
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert all(torch.equal(i, j) for i, j in zip(out, want))
+    assert capi.read_device_error() == 0
+
+
+@gpu
+def test_gradients_accumulate_and_chain():
+    """A feed-forward block as it would be used: two layers, the skip connection in the second's epilogue, shared weights."""
+    dtype = torch.float16
+    torch.manual_seed(0)
+    up = lin.Linear(64, 256, activation="gelu", checkpoint="e4m3", dtype=dtype).cuda()
+    down = lin.Linear(256, 64, dtype=dtype).cuda()
+    x = (torch.randn(50, 64, device="cuda") * 0.5).to(dtype).requires_grad_()
+    for _ in range(2):
+        h = x
+        for _ in range(2):                       # the same weights twice: gradients of both uses add up
+            h = down(up(h), h)
+        h.float().square().mean().backward()
+    names = [x, *up.parameters(), *down.parameters()]
+    got = [t.grad.double() / 2 for t in names]
+    ref = [t.detach().double().requires_grad_() for t in names]
+    h = ref[0]
+    for _ in range(2):
+        h = F.linear(F.gelu(F.linear(h, ref[1], ref[2])), ref[3], ref[4]) + h
+    h.square().mean().backward()
+    for g, t in zip(got, ref):
+        # four significant bits of x and z: 2^-4 of each at most, a third of that in the mean square of many
+        assert (g - t.grad).norm() <= 2.0 ** -4 * t.grad.norm()
+
+
+@gpu
+def test_module_follows_its_parameters():
+    layer = lin.Linear(40, 24, activation="relu").cuda()
+    ref = torch.nn.Linear(40, 24).cuda()
+    ref.load_state_dict(layer.state_dict())
+    x = torch.randn(10, 40, device="cuda", requires_grad=True)
+    y = layer(x)
+    assert y.dtype == torch.float16
+    z64 = F.linear(x.detach().half().double(), layer.weight.detach().half().double(), layer.bias.detach().double())
+    assert ((y.double() - F.relu(z64)).abs() <= half_step(z64, torch.float16) + 2.0 ** -20).all()
+    y.float().sum().backward()
+    assert x.grad.dtype == torch.float32 and layer.weight.grad.dtype == torch.float32 and layer.bias.grad.dtype == torch.float32
+    with torch.no_grad():
+        layer.weight.zero_()
+        layer.bias.fill_(0.5)
+    assert (layer(x) == 0.5).all()
+    assert lin.Linear(8, 8, compute_dtype=None, dtype=torch.bfloat16).cuda()(torch.ones(2, 8, device="cuda", dtype=torch.bfloat16)).dtype == torch.bfloat16
+    assert "activation=relu" in repr(layer)
+
+
+@gpu
+def test_refusals_on_the_device():
+    x, w, b, r = make(4, 16, 24, torch.float16)
+    for args, kw, text in (((x.float(), w), {}, "float16 or bfloat16"), ((x, w[:, :8]), {}, "input features"), ((x, w.bfloat16()), {}, "weight must be"),
+                           ((x, w, b[:8]), {}, "bias must be"), ((x, w, b.double()), {}, "bias must be"), ((x, w, b, r[:1]), {}, "residual must have"),
+                           ((x, w, b, r.float()), {}, "residual must be"), ((x, w.cpu()), {}, "weight is on"), ((x, w, b.cpu()), {}, "bias is on"),
+                           ((x, w[:0]), {}, "not be empty"), ((x, w[0]), {}, "weight must be")):
+        with pytest.raises(RuntimeError, match=text):
+            lin.linear(*args, **kw)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        leaf = x.clone().requires_grad_()
+        torch.autograd.grad(lin.linear(leaf, w).float().sum(), leaf, create_graph=True)
+    leaf = x.clone().requires_grad_()
+    wl = w.clone().requires_grad_()
+    y = lin.linear(leaf * 1, wl)
+    with torch.no_grad():
+        wl.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.float().sum().backward()
+
+
+# ---- without a GPU -------------------------------------------------------------------------------------------------------
+def test_refusals_of_the_python_layer():
+    x, w = torch.zeros(2, 8, dtype=torch.float16), torch.zeros(4, 8, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        lin.linear(x, w)
+    with pytest.raises(ValueError, match="activation must be one of"):
+        lin.linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="checkpoint must be"):
+        lin.linear(x, w, checkpoint="int8")
+    with pytest.raises(ValueError, match="compute_dtype"):
+        lin.Linear(8, 8, compute_dtype=torch.float32)
+    with pytest.raises(ValueError, match="activation"):
+        lin.Linear(8, 8, activation=["relu"])
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        checkpoint.pack(x)
+    with pytest.raises(RuntimeError, match="CUDA devices only"):
+        checkpoint.unpack(x.to(torch.float8_e4m3fn), torch.zeros(2, 1, dtype=torch.uint8).view(torch.float8_e8m0fnu))
+    layer = lin.Linear(8, 4, activation="silu", checkpoint="e4m3")
+    assert list(layer.state_dict()) == list(torch.nn.Linear(8, 4).state_dict())
+
+
+def test_refusals_of_the_c_abi():
+    lib = capi.lib()
+    p = 1 << 20      # never dereferenced: every call is refused before a launch
+
+    def desc(**kw):
+        return ctypes.byref(capi.LinearDesc(**{**dict(rows=4, in_features=16, out_features=24, dtype=capi.F16), **kw}))
+
+    def fwd(d, x=p, w=p, bias=None, res=None, y=p, z=None, z8=None, zs=None):
+        return lib.winoconv_linear_forward(d, x, w, bias, res, y, z, z8, zs, None)
+
+    bad, unsupported = capi.ERR_INVALID_ARGUMENT, capi.ERR_UNSUPPORTED
+    for status, want in ((fwd(None), bad), (fwd(desc(dtype=capi.F32)), unsupported), (fwd(desc(activation=5)), bad), (fwd(desc(activation=-1)), bad),
+                         (fwd(desc(rows=0)), bad), (fwd(desc(in_features=-1)), bad), (fwd(desc(out_features=0)), bad),
+                         (fwd(desc(rows=1 << 33)), unsupported), (fwd(desc(rows=(1 << 31) - 2000, out_features=(1 << 31) - 2000)), unsupported),
+                         (fwd(desc(x_stride=8)), bad), (fwd(desc(y_stride=23)), bad), (fwd(desc(z_stride=1)), bad), (fwd(desc(residual_stride=1)), bad),
+                         (fwd(desc(x_stride=17)), bad), (fwd(desc(w_stride=20)), bad), (fwd(desc(in_features=15)), bad), (fwd(desc(x_stride=1 << 40)), unsupported),
+                         (fwd(desc(), x=None), bad), (fwd(desc(), w=None), bad), (fwd(desc(), y=None), bad), (fwd(desc(), x=p + 8), bad),
+                         (fwd(desc(), w=p + 2), bad), (fwd(desc(), y=p + 1), bad), (fwd(desc(), bias=p + 1), bad), (fwd(desc(bias_f32=1), bias=p + 2), bad),
+                         (fwd(desc(), res=p + 1), bad), (fwd(desc(), z=p + 1), bad), (fwd(desc(), z8=p), bad), (fwd(desc(), zs=p), bad),
+                         (fwd(desc(), z8=p + 8, zs=p), bad)):
+        assert status == want, capi.last_error()
+
+    def act(d, gy=p, gs=0, z=None, z8=None, zs=None, dz=p, dzs=0, db=None, dbt=0, ws=None, n=0):
+        return lib.winoconv_linear_backward_activation(d, gy, gs, z, z8, zs, dz, dzs, db, dbt, ws, n, None)
+
+    relu = desc(activation=1)
+    for status, want in ((act(relu), bad), (act(relu, z=p, z8=p, zs=p), bad), (act(relu, z8=p), bad), (act(relu, z=p, gy=None), bad), (act(relu, z=p, dz=None), bad),
+                         (act(relu, z=p, gs=3), bad), (act(relu, z=p, dzs=3), bad), (act(relu, z=p, db=p, dbt=9, ws=p, n=1 << 20), bad),
+                         (act(relu, z=p, db=p), bad), (act(relu, z=p, db=p, ws=p, n=8), capi.ERR_WORKSPACE), (act(relu, z=p + 1), bad), (act(relu, z=p, gy=p + 1), bad)):
+        assert status == want, capi.last_error()
+    need = ctypes.c_uint64(0)
+    assert lib.winoconv_linear_backward_ws(desc(), ctypes.byref(need)) == capi.OK and need.value >= 24 * 4
+    assert lib.winoconv_linear_backward_ws(desc(), None) == bad
+    data, weight = lib.winoconv_linear_backward_data, lib.winoconv_linear_backward_weight
+    for status, want in ((data(desc(), p, 0, p, None, 0, None), bad), (data(desc(), p + 2, 0, p, p, 0, None), bad), (data(desc(), p, 25, p, p, 0, None), bad),
+                         (data(desc(), p, 0, p, p, 8, None), bad), (data(desc(out_features=23), p, 0, p, p, 0, None), bad), (data(desc(), p, 0, None, p, 0, None), bad),
+                         (weight(desc(), p, 0, p, None, 0, None), bad), (weight(desc(), p, 0, p, p, capi.BF16, None), unsupported),
+                         (weight(desc(), p, 0, p + 4, p, 0, None), bad), (weight(desc(), p, 0, p, p + 2, 0, None), bad)):
+        assert status == want, capi.last_error()
+    pad = lib.winoconv_pad_rows
+    for status, want in ((pad(None, 0, p, 8, 1, 8, None), bad), (pad(p, 0, p, 9, 1, 8, None), bad), (pad(p, 0, p, 8, 1, 9, None), bad), (pad(p, 0, p + 8, 8, 1, 8, None), bad),
+                         (pad(p, 4, p, 8, 1, 8, None), bad), (pad(p, 0, p, 8, 0, 8, None), bad), (pad(p + 1, 0, p, 8, 1, 8, None), bad)):
+        assert status == want, capi.last_error()
+
+
+def test_the_c_abi_reports_a_missing_device():
+    if torch.cuda.is_available():
+        pytest.skip("a device is there")
+    p = 1 << 20
+    d = capi.LinearDesc(rows=4, in_features=16, out_features=24, dtype=capi.F16)
+    assert capi.lib().winoconv_linear_forward(ctypes.byref(d), p, p, None, None, p, None, None, None, None) == capi.ERR_NO_DEVICE
