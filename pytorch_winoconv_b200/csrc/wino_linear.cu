@@ -55,11 +55,20 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap *map
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1) : "memory");
 }
+// The same of a CTA pair: each CTA fills its own shared memory, the bytes are counted on rank 0's barrier.
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar & RANK0_MASK), "r"(c0), "r"(c1) : "memory");
+}
 // `n` rows from `row` on, reduction from `k` on: one box, or a box per 64 rows where the rows lie contiguous.
-__device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap *map, uint32_t bar, int mn, int row, int n, int k) {
-  if (!mn) tma_load_2d(dst, map, bar, k, row);
+template <bool PAIR> __device__ __forceinline__ void load_operand(uint32_t dst, const CUtensorMap *map, uint32_t bar, int mn, int row, int n, int k) {
+  auto load = [&](uint32_t to, int c0, int c1) {
+    if (PAIR) tma_load_2d_pair(to, map, bar, c0, c1);
+    else tma_load_2d(to, map, bar, c0, c1);
+  };
+  if (!mn) load(dst, k, row);
   else
-    for (int j = 0; j < n; j += 64) tma_load_2d(dst + (uint32_t)j * 128u, map, bar, row + j, k);
+    for (int j = 0; j < n; j += 64) load(dst + (uint32_t)j * 128u, row + j, k);
 }
 // Low descriptor word of an operand tile and the step between its 16-value slices (16-byte units).  MN-major: blocks of 64 rows
 // 8 KB apart, groups of eight reduction steps 1 KB apart; K-major: groups of eight rows 1 KB apart.
@@ -199,8 +208,8 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
       if (lane == 0) {
         mbar_expect_tx(full(s), stage_bytes);
         const uint32_t dst = base + (uint32_t)s * stage_bytes;
-        load_operand(dst, &map_c, full(s), g.c_mn, col0, BC, k * BK);
-        load_operand(dst + C_BYTES, &map_r, full(s), g.r_mn, row0, g.tile_rows, k * BK);
+        load_operand<false>(dst, &map_c, full(s), g.c_mn, col0, BC, k * BK);
+        load_operand<false>(dst + C_BYTES, &map_r, full(s), g.r_mn, row0, g.tile_rows, k * BK);
       }
       if (++s == g.stages) { s = 0; ph ^= 1u; }
     }
@@ -282,6 +291,286 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   }
 }
 
+// ---- pair kernel -----------------------------------------------------------------------------------------------------
+constexpr int PAIR_THREADS = 384, PAIR_STAGES = 6;
+constexpr int PAIR_TILE = 256;                                    // rows and columns of a tile; a CTA holds half of each operand
+constexpr int PAIR_STAGE = 2 * 128 * BK * 2;                      // bytes a CTA loads for a stage
+constexpr int PAIR_WARPS = 8;                                     // of the epilogue
+constexpr int TURN_BYTES = 2048, BIAS_BYTES = 512;                // per epilogue warp: 32 rows x 64 bytes, 128 bias values
+constexpr int PAIR_OFF_TURN = PAIR_STAGES * PAIR_STAGE, PAIR_OFF_BIAS = PAIR_OFF_TURN + PAIR_WARPS * TURN_BYTES,
+              PAIR_OFF_BARS = PAIR_OFF_BIAS + PAIR_WARPS * BIAS_BYTES, PAIR_SMEM = 1024 + PAIR_OFF_BARS + BAR_BYTES;
+static_assert(PAIR_SMEM <= 227 * 1024, "shared memory");
+
+struct PairArgs {
+  int n_steps, n_rt, n_ct, n_tiles, r_mn, c_mn;
+  uint32_t idesc;
+};
+// Tiles are walked in bands of eight tile rows, column by column: the pairs at work at one time share few rows and few columns,
+// which then come from L2.
+constexpr int BAND = 8;
+__device__ __forceinline__ void tile_at(const PairArgs &g, int t, int &rt, int &ct) {
+  const int per = BAND * g.n_ct, band = t / per, r = t - band * per, n = min(BAND, g.n_rt - band * BAND);
+  ct = r / n;
+  rt = band * BAND + (r - ct * n);
+}
+
+// 64 bytes of each of a warp's 32 rows (lane = row), turned in shared memory so that the stores of a row are contiguous.  EL:
+// bytes of an element; `rows` and `cols` are what is left of the matrix from here on.
+template <int EL>
+__device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16], uint8_t *dst, long long stride, int rows, int cols, int wide, int lane) {
+  uint4 *mine = reinterpret_cast<uint4 *>(turn + lane * 64);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mine[i ^ ((lane >> 1) & 3)] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+  __syncwarp();
+  if (wide) {
+    const int c = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 8 + (lane >> 2);
+      const uint4 v = *reinterpret_cast<const uint4 *>(turn + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+      if (r < rows && c * (16 / EL) < cols) *reinterpret_cast<uint4 *>(dst + r * stride + c * 16) = v;
+    }
+  } else {
+    constexpr int PER = 64 / EL, RS = 32 / PER;      // elements of a row, rows a time
+    const int c = lane % PER;
+    for (int r = lane / PER; r < min(32, rows); r += RS) {
+      const uint8_t *src = turn + r * 64 + ((((c * EL) >> 4) ^ ((r >> 1) & 3)) << 4) + ((c * EL) & 15);
+      if (c < cols) {
+        if constexpr (EL == 2) *reinterpret_cast<uint16_t *>(dst + r * stride + c * 2) = *reinterpret_cast<const uint16_t *>(src);
+        else *reinterpret_cast<uint32_t *>(dst + r * stride + c * 4) = *reinterpret_cast<const uint32_t *>(src);
+      }
+    }
+  }
+  __syncwarp();
+}
+// The counterpart for 16-bit rows that take no vectors: 32 columns of each row, as the lane that holds the row wants them.
+__device__ __forceinline__ void load_rows(uint8_t *turn, uint32_t (&w)[16], const uint8_t *src, long long stride, int rows, int cols, int lane) {
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r) {
+    const uint16_t v = r < rows && lane < cols ? *reinterpret_cast<const uint16_t *>(src + r * stride + lane * 2) : (uint16_t)0;
+    *reinterpret_cast<uint16_t *>(turn + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2) = v;
+  }
+  __syncwarp();
+  const uint4 *mine = reinterpret_cast<const uint4 *>(turn + lane * 64);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 v = mine[i ^ ((lane >> 1) & 3)];
+    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+  }
+  __syncwarp();
+}
+
+// ACT: the activation of a layer; -1: the product alone.
+template <typename T, int ACT>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Out o,
+                const __grid_constant__ PairArgs g) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t *base_ptr = smem_raw + (base - raw);
+  const uint32_t bars = base + PAIR_OFF_BARS;      // full[6] empty[6] acc_full[2] acc_empty[2]
+  auto full = [&](int i) { return bars + 8u * i; };
+  auto empty = [&](int i) { return bars + 64u + 8u * i; };
+  auto acc_full = [&](int i) { return bars + 128u + 8u * i; };
+  auto acc_empty = [&](int i) { return bars + 144u + 8u * i; };
+  const uint32_t tmem_slot = bars + 196u;
+  volatile unsigned *abort_word = reinterpret_cast<volatile unsigned *>(base_ptr + PAIR_OFF_BARS + 192);
+  unsigned *err = &g_linear_error;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+
+  if (warp == 1 && lane == 0) { prefetch_map(&map_r); prefetch_map(&map_c); }
+  if (warp == 0) {
+    if (lane < PAIR_STAGES) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
+    else if (lane < 8) { mbar_init(acc_full(lane - 6), 1); mbar_init(acc_empty(lane - 6), 2 * PAIR_WARPS); }
+    else if (lane == 8) *abort_word = 0u;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;                   // issues the MMAs of the pair
+  if (warp == 2) tmem_alloc<true>(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                              // the barriers of both CTAs exist before either arrives at the other's
+  tc_fence_after();
+  uint32_t tmem;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
+  tmem = __shfl_sync(0xffffffffu, tmem, 0);
+  grid_launch_dependents();
+  grid_dependency_wait();
+
+  const int tile0 = (int)blockIdx.x >> 1, tile_step = (int)gridDim.x >> 1;
+  if (warp == 0) {
+    int s = 0;
+    uint32_t ph = 1;
+    bool alive = true;
+    for (int t = tile0; t < g.n_tiles && alive; t += tile_step) {
+      int rt, ct;
+      tile_at(g, t, rt, ct);
+      const int row = rt * PAIR_TILE + (int)rank * 128, col = ct * PAIR_TILE + (int)rank * 128;
+      for (int k = 0; k < g.n_steps; ++k) {
+        if (!mbar_wait_warp(empty(s), ph, abort_word, err, ERR_EMPTY)) { alive = false; break; }
+        if (lane == 0) {
+          if (leader) mbar_expect_tx(full(s), 2u * PAIR_STAGE);
+          const uint32_t dst = base + (uint32_t)(s * PAIR_STAGE);
+          load_operand<true>(dst, &map_r, full(s), g.r_mn, row, 128, k * BK);
+          load_operand<true>(dst + PAIR_STAGE / 2, &map_c, full(s), g.c_mn, col, 128, k * BK);
+        }
+        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+      }
+    }
+    if (*abort_word != 0u) {   // loads in flight must land before the shared memory goes away
+      const long long start = clock64();
+      while (clock64() - start < 2000000LL) { }
+    }
+  } else if (warp == 1 && leader) {
+    int s = 0, n = 0;
+    uint32_t ph = 0;
+    bool alive = true;
+    const uint32_t hi = desc_hi(1024, 2), a_step = operand_step(g.r_mn), b_step = operand_step(g.c_mn);
+    for (int t = tile0; t < g.n_tiles && alive; t += tile_step, ++n) {
+      const int buf = n & 1;
+      if (!mbar_wait_warp(acc_empty(buf), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_word, err, ERR_ACC_EMPTY)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + (uint32_t)(buf * PAIR_TILE);
+      for (int k = 0; k < g.n_steps; ++k) {
+        if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
+        tc_fence_after();
+        const uint32_t st = base + (uint32_t)(s * PAIR_STAGE);
+        const uint32_t a = operand_lo(st, g.r_mn), b = operand_lo(st + PAIR_STAGE / 2, g.c_mn);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) umma<true, false>(d, a + (uint32_t)j * a_step, hi, b + (uint32_t)j * b_step, hi, g.idesc, (k > 0 || j > 0) ? 1u : 0u);
+          umma_commit<true>(empty(s), 3);
+        }
+        __syncwarp();
+        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+      }
+      if (alive && elect_one()) umma_commit<true>(acc_full(buf), 3);
+      __syncwarp();
+    }
+  } else if (warp >= 4) {
+    const int ew = warp - 4, q = warp & 3, half = ew >> 2;
+    uint8_t *turn = base_ptr + PAIR_OFF_TURN + ew * TURN_BYTES;
+    float *bias = reinterpret_cast<float *>(base_ptr + PAIR_OFF_BIAS + ew * BIAS_BYTES);
+    const int n_blk = (o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK;
+    int n = 0;
+    for (int t = tile0; t < g.n_tiles; t += tile_step, ++n) {
+      int rt, ct;
+      tile_at(g, t, rt, ct);
+      const int buf = n & 1;
+      const int row0 = rt * PAIR_TILE + (int)rank * 128 + q * 32, col0 = ct * PAIR_TILE + half * 128, rows = o.rows - row0;
+      if (ACT >= 0) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int c = col0 + j * 32 + lane;
+          bias[j * 32 + lane] = !o.bias || c >= o.cols ? 0.f : o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[c] : Elem<T>::load((const T *)o.bias + c);
+        }
+        __syncwarp();
+      }
+      if (!mbar_wait_warp(acc_full(buf), (uint32_t)(n >> 1) & 1u, abort_word, err, ERR_ACC_FULL)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int ch = 0; ch < 4; ++ch) {
+        const int c = col0 + ch * 32, cols = o.cols - c;
+        if (cols <= 0 || rows <= 0) break;
+        uint32_t v[32];
+        tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_TILE + half * 128 + ch * 32), v);
+        uint32_t res[16];
+        if (ACT >= 0 && o.residual) {      // on its way while the accumulator is read
+          const uint8_t *src = (const uint8_t *)o.residual + ((long long)row0 * o.residual_stride + c) * 2;
+          if (o.wide) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint4 u = make_uint4(0u, 0u, 0u, 0u);
+              if (lane < rows && i * 8 < cols) u = *reinterpret_cast<const uint4 *>(src + lane * o.residual_stride * 2 + i * 16);
+              res[4 * i] = u.x; res[4 * i + 1] = u.y; res[4 * i + 2] = u.z; res[4 * i + 3] = u.w;
+            }
+          } else load_rows(turn, res, src, o.residual_stride * 2, rows, cols, lane);
+        }
+        tmem_wait_ld_x32(v);
+        float f[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
+        uint32_t w[16];
+        if constexpr (ACT >= 0) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 b = *reinterpret_cast<const float4 *>(bias + ch * 32 + i * 4);
+            f[4 * i] += b.x; f[4 * i + 1] += b.y; f[4 * i + 2] += b.z; f[4 * i + 3] += b.w;
+          }
+          if (o.z) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = Pair16<T>::round(f[2 * i], f[2 * i + 1]);
+            store_rows<2>(turn, w, (uint8_t *)o.z + ((long long)row0 * o.z_stride + c) * 2, o.z_stride * 2, rows, cols, o.wide, lane);
+          }
+          if (o.z8) {      // a lane's 32 columns are a block (columns beyond the last are zero)
+            float top = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) top = fmaxf(top, e4m3::finite_magnitude(f[i]));
+            const uint32_t byte = e4m3::scale_byte(top);
+            const float inv = e4m3::inverse_scale(byte);
+            uint32_t p[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) p[i] = e4m3::pack2(f[4 * i], f[4 * i + 1], inv) | (e4m3::pack2(f[4 * i + 2], f[4 * i + 3], inv) << 16);
+            uint8_t *dst = o.z8 + (long long)row0 * o.cols + c;
+            if ((o.cols & 15) == 0) {
+              if (lane < rows) {
+                uint4 *d4 = reinterpret_cast<uint4 *>(dst + (long long)lane * o.cols);
+                d4[0] = make_uint4(p[0], p[1], p[2], p[3]);
+                if (cols > 16) d4[1] = make_uint4(p[4], p[5], p[6], p[7]);
+              }
+            } else {
+              uint4 *mine = reinterpret_cast<uint4 *>(turn + lane * 32);
+              mine[0] = make_uint4(p[0], p[1], p[2], p[3]);
+              mine[1] = make_uint4(p[4], p[5], p[6], p[7]);
+              __syncwarp();
+              for (int r = 0; r < min(32, rows); ++r)
+                if (lane < cols) dst[(long long)r * o.cols + lane] = turn[r * 32 + lane];
+              __syncwarp();
+            }
+            if (lane < rows) o.z8_scale[(long long)(row0 + lane) * n_blk + c / e4m3::BLOCK] = (uint8_t)byte;
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) f[i] = act::apply(f[i], ACT);
+          if (o.residual) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 r = Pair16<T>::unpack(res[i]);
+              f[2 * i] += r.x;
+              f[2 * i + 1] += r.y;
+            }
+          }
+        }
+        if (ACT < 0 && o.out_f32) {
+          uint8_t *dst = (uint8_t *)o.y + ((long long)row0 * o.y_stride + c) * 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(f[16 * h + i]);
+            store_rows<4>(turn, w, dst + h * 64, o.y_stride * 4, rows, cols - 16 * h, o.wide, lane);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = Pair16<T>::round(f[2 * i], f[2 * i + 1]);
+          store_rows<2>(turn, w, (uint8_t *)o.y + ((long long)row0 * o.y_stride + c) * 2, o.y_stride * 2, rows, cols, o.wide, lane);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_rank0(acc_empty(buf));
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_free<true>(tmem, 512);
+  }
+}
+
 // Boxes of 64 x `rows` (K-major) or 64 rows x 64 reduction steps (MN-major), zeros beyond the operand's ends.
 bool operand_map(CUtensorMap *m, EncodeTiledFn enc, int dtype, const MatOperand &p, int rows, int red, int box_rows) {
   cuuint64_t dims[2] = {(cuuint64_t)(p.mn ? rows : red), (cuuint64_t)(p.mn ? red : rows)}, st[1] = {(cuuint64_t)p.stride * 2};
@@ -356,6 +645,45 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
   return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 4), g, plan.split);
 }
 
+template <typename T, int ACT>
+cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  CUtensorMap mr, mc;
+  if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, 128) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, 128)) {
+    *detail = "cuTensorMapEncodeTiled failed";
+    return cudaErrorInvalidValue;
+  }
+  auto kern = pair_kernel<T, ACT>;
+  cudaError_t e = allow_smem((const void *)kern);
+  if (e != cudaSuccess) return e;
+  PairArgs g;
+  g.n_steps = (p.red + BK - 1) / BK;
+  g.n_rt = (p.rows + PAIR_TILE - 1) / PAIR_TILE; g.n_ct = (p.cols + PAIR_TILE - 1) / PAIR_TILE;
+  g.n_tiles = g.n_rt * g.n_ct;
+  g.r_mn = p.r.mn; g.c_mn = p.c.mn;
+  g.idesc = instruction(p.dtype, p.r.mn, p.c.mn, 256, 256);
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(PAIR_THREADS);
+  cfg.dynamicSmemBytes = PAIR_SMEM; cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  cfg.gridDim = dim3(2u * (unsigned)std::min(g.n_tiles, SMS / 2));
+  return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 8), g);
+}
+template <typename T> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  if (!p.layer) return launch_pair<T, -1>(p, enc, s, detail);
+  switch (p.act) {
+    case WINOCONV_ACT_RELU: return launch_pair<T, WINOCONV_ACT_RELU>(p, enc, s, detail);
+    case WINOCONV_ACT_GELU: return launch_pair<T, WINOCONV_ACT_GELU>(p, enc, s, detail);
+    case WINOCONV_ACT_GELU_TANH: return launch_pair<T, WINOCONV_ACT_GELU_TANH>(p, enc, s, detail);
+    case WINOCONV_ACT_SILU: return launch_pair<T, WINOCONV_ACT_SILU>(p, enc, s, detail);
+    default: return launch_pair<T, WINOCONV_ACT_NONE>(p, enc, s, detail);
+  }
+}
+
 }  // namespace linear
 
 using namespace linear;
@@ -364,6 +692,9 @@ using namespace linear;
 // bring the grid nearest to two on every SM from below.
 LinearPlan linear_plan(const LinearProblem &p) {
   LinearPlan plan = {};
+  const long long pair_tiles = (long long)((p.rows + PAIR_TILE - 1) / PAIR_TILE) * ((p.cols + PAIR_TILE - 1) / PAIR_TILE);
+  plan.pair = p.rows > 128 && pair_tiles >= 32;
+  if (plan.pair) return plan;
   const int unit = p.r.mn ? 64 : 16;
   plan.tile_rows = std::min(128, (p.rows + unit - 1) / unit * unit);
   const long long tiles = (long long)((p.rows + plan.tile_rows - 1) / plan.tile_rows) * ((p.cols + BC - 1) / BC);
@@ -379,6 +710,7 @@ cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaSt
   *detail = "";
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
+  if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, enc, s, detail) : launch_pair<__nv_bfloat16>(p, enc, s, detail);
   return p.dtype == WINOCONV_F16 ? launch_cluster<__half>(p, plan, enc, s, detail) : launch_cluster<__nv_bfloat16>(p, plan, enc, s, detail);
 }
 
