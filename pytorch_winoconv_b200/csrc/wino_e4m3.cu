@@ -25,41 +25,79 @@ __device__ __forceinline__ void split_index(unsigned long long i, unsigned per, 
   }
 }
 
+// Where item `i` of eight values lies: in rows x_stride apart, among the eight-bit rows, and its block.  FLAT: rows without gaps
+// and of whole blocks, no division by a row's length.
+template <bool FLAT>
+__device__ __forceinline__ bool place(unsigned long long i, unsigned long long n_items, unsigned per_row, int cols, long long x_stride, long long &wide,
+                                      long long &dense, long long &block) {
+  if constexpr (FLAT) {
+    wide = dense = (long long)(i * 8);
+    block = (long long)(i >> 2);
+    return i < n_items;
+  } else {
+    long long row;
+    unsigned at;
+    split_index(i, per_row, row, at);
+    wide = row * x_stride + at * 8;
+    dense = row * cols + at * 8;
+    block = row * (per_row >> 2) + (at >> 2);
+    return i < n_items && (int)(at * 8) < cols;
+  }
+}
+// The kernels start while the one before them ends (programmatic dependent launch): nothing is read or written before this.
+__device__ __forceinline__ void grid_start() {
+  sm100::grid_launch_dependents();
+  sm100::grid_dependency_wait();
+}
+
 // Items of eight values, four lanes to a block.
-template <typename T>
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(THREADS) pack_kernel(const T *__restrict__ x, long long x_stride, uint8_t *__restrict__ q, uint8_t *__restrict__ scale,
                                                        unsigned long long n_items, unsigned per_row, int cols) {
   const unsigned long long i0 = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
   uint4 v[UNROLL];
-  long long row[UNROLL];
-  unsigned at[UNROLL];
+  long long to[UNROLL], block[UNROLL];
   bool in[UNROLL];
+  grid_start();
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned long long i = i0 + u * THREADS;
-    split_index(i, per_row, row[u], at[u]);
-    in[u] = i < n_items && (int)(at[u] * 8) < cols;
-    v[u] = in[u] ? *reinterpret_cast<const uint4 *>(x + row[u] * x_stride + at[u] * 8) : make_uint4(0u, 0u, 0u, 0u);
+    long long from;
+    in[u] = place<FLAT>(i, n_items, per_row, cols, x_stride, from, to[u], block[u]);
+    v[u] = in[u] ? *reinterpret_cast<const uint4 *>(x + from) : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-    float f[8], top = 0.f;
+    uint32_t m = 0u;      // (a packed maximum leaves NaN out)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) m = Pair16<T>::max2(m, w[j] & 0x7FFF7FFFu);
+    m = Pair16<T>::max2(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = Pair16<T>::max2(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const float2 m2 = Pair16<T>::unpack(m);
+    float f[8], top = fmaxf(m2.x, m2.y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float2 p = Pair16<T>::unpack(w[j]);
       f[2 * j] = p.x;
       f[2 * j + 1] = p.y;
-      top = fmaxf(top, fmaxf(finite_magnitude(p.x), finite_magnitude(p.y)));
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    if (__any_sync(0xffffffffu, top == __uint_as_float(0x7F800000u))) {      // rare: an infinity takes no part in the scale and is kept as NaN
+      top = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        top = fmaxf(top, finite_magnitude(f[j]));
+        f[j] = fabsf(f[j]) < __uint_as_float(0x7F800000u) ? f[j] : __uint_as_float(0x7FC00000u);
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    }
     const uint32_t byte = scale_byte(top);
     const float inv = inverse_scale(byte);
-    const uint2 r = make_uint2(pack2(f[0], f[1], inv) | (pack2(f[2], f[3], inv) << 16), pack2(f[4], f[5], inv) | (pack2(f[6], f[7], inv) << 16));
+    const uint2 r = make_uint2(pack2_finite(f[0], f[1], inv) | (pack2_finite(f[2], f[3], inv) << 16), pack2_finite(f[4], f[5], inv) | (pack2_finite(f[6], f[7], inv) << 16));
     if (in[u]) {
-      *reinterpret_cast<uint2 *>(q + row[u] * cols + at[u] * 8) = r;
-      if ((threadIdx.x & 3) == 0) scale[row[u] * (per_row >> 2) + (at[u] >> 2)] = (uint8_t)byte;
+      *reinterpret_cast<uint2 *>(q + to[u]) = r;
+      if ((threadIdx.x & 3) == 0) scale[block[u]] = (uint8_t)byte;
     }
   }
 }
@@ -74,6 +112,7 @@ __global__ void __launch_bounds__(THREADS) pack_ragged_kernel(const T *__restric
   long long row[UNROLL];
   unsigned at[UNROLL];
   bool in[UNROLL];
+  grid_start();
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned long long b = b0 + u * (THREADS / 32);
@@ -94,38 +133,42 @@ __global__ void __launch_bounds__(THREADS) pack_ragged_kernel(const T *__restric
   }
 }
 
-template <typename T> __device__ __forceinline__ uint32_t values2(uint32_t q, float s) {
-  const float2 f = unpack2(q);
-  return Pair16<T>::round(within<T>(f.x * s), within<T>(f.y * s));
+// Four values in 16 bits; only a block with the largest scales can reach beyond the type.
+template <typename T> __device__ __forceinline__ uint2 values4(uint32_t q, uint32_t byte, float s) {
+  float2 a = unpack2(q & 0xFFFFu), b = unpack2(q >> 16);
+  a.x *= s; a.y *= s; b.x *= s; b.y *= s;
+  if (byte > safe_byte<T>()) { a.x = within<T>(a.x); a.y = within<T>(a.y); b.x = within<T>(b.x); b.y = within<T>(b.y); }
+  return make_uint2(Pair16<T>::round(a.x, a.y), Pair16<T>::round(b.x, b.y));
 }
 
-template <typename T>
+template <typename T, bool FLAT>
 __global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ scale, T *__restrict__ x,
                                                          long long x_stride, unsigned long long n_items, unsigned per_row, int cols) {
   const unsigned long long i0 = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
   uint2 v[UNROLL];
   uint32_t byte[UNROLL];
-  long long row[UNROLL];
-  unsigned at[UNROLL];
+  long long to[UNROLL];
   bool in[UNROLL];
+  grid_start();
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned long long i = i0 + u * THREADS;
-    split_index(i, per_row, row[u], at[u]);
-    in[u] = i < n_items && (int)(at[u] * 8) < cols;
+    long long from, block;
+    in[u] = place<FLAT>(i, n_items, per_row, cols, x_stride, to[u], from, block);
     v[u] = make_uint2(0u, 0u);
     byte[u] = 0u;
     if (in[u]) {
-      v[u] = *reinterpret_cast<const uint2 *>(q + row[u] * cols + at[u] * 8);
-      byte[u] = scale[row[u] * (per_row >> 2) + (at[u] >> 2)];
+      v[u] = *reinterpret_cast<const uint2 *>(q + from);
+      byte[u] = scale[block];
     }
   }
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const float s = scale_of(byte[u]);
-    if (in[u])
-      *reinterpret_cast<uint4 *>(x + row[u] * x_stride + at[u] * 8) =
-          make_uint4(values2<T>(v[u].x & 0xFFFFu, s), values2<T>(v[u].x >> 16, s), values2<T>(v[u].y & 0xFFFFu, s), values2<T>(v[u].y >> 16, s));
+    if (in[u]) {
+      const uint2 a = values4<T>(v[u].x, byte[u], s), b = values4<T>(v[u].y, byte[u], s);
+      *reinterpret_cast<uint4 *>(x + to[u]) = make_uint4(a.x, a.y, b.x, b.y);
+    }
   }
 }
 
@@ -134,6 +177,7 @@ __global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *_
                                                                 long long x_stride, unsigned long long n_blocks, unsigned per_row, int cols) {
   const int lane = threadIdx.x & 31;
   const unsigned long long b0 = (unsigned long long)blockIdx.x * (THREADS / 32 * UNROLL) + (threadIdx.x >> 5);
+  grid_start();
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned long long b = b0 + u * (THREADS / 32);
@@ -150,6 +194,7 @@ __global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *_
 // Rows copied with zeros behind them; T is any 16-bit type.
 __global__ void __launch_bounds__(THREADS) pad_rows_kernel(const uint16_t *__restrict__ x, long long x_stride, uint16_t *__restrict__ y, long long out_stride,
                                                            unsigned long long n_items, unsigned per_row, int cols) {
+  grid_start();
 #pragma unroll
   for (int u = 0; u < UNROLL; ++u) {
     const unsigned long long i = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x + u * THREADS;
@@ -169,61 +214,92 @@ __global__ void __launch_bounds__(THREADS) pad_rows_kernel(const uint16_t *__res
 // every time.
 constexpr int ROWS = 8;
 
-template <typename T, int V> struct Run {
-  static __device__ __forceinline__ void load(const T *p, float (&f)[V]) {
-    if constexpr (V == 8) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(p);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+template <typename T, int V> struct Run;
+template <typename T> struct Run<T, 8> {
+  using Raw = uint4;
+  using Raw8 = uint2;
+  static __device__ __forceinline__ void values(const uint4 &v, float (&f)[8]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 t = Pair16<T>::unpack(w[j]);
-        f[2 * j] = t.x;
-        f[2 * j + 1] = t.y;
-      }
-    } else f[0] = Elem<T>::load(p);
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = Pair16<T>::unpack(w[j]);
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
+    }
   }
-  static __device__ __forceinline__ void store(T *p, const float (&f)[V]) {
-    if constexpr (V == 8)
-      *reinterpret_cast<uint4 *>(p) = make_uint4(Pair16<T>::round(f[0], f[1]), Pair16<T>::round(f[2], f[3]), Pair16<T>::round(f[4], f[5]), Pair16<T>::round(f[6], f[7]));
-    else Elem<T>::store(p, f[0]);
+  static __device__ __forceinline__ void values8(const uint2 &v, uint32_t byte, float (&f)[8]) {
+    const float s = scale_of(byte);
+    const uint32_t w[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = unpack2(w[j]);
+      f[2 * j] = t.x * s;
+      f[2 * j + 1] = t.y * s;
+    }
+    if (byte > safe_byte<T>()) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = within<T>(f[j]);
+    }
+  }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[8]) {
+    *reinterpret_cast<uint4 *>(p) = make_uint4(Pair16<T>::round(f[0], f[1]), Pair16<T>::round(f[2], f[3]), Pair16<T>::round(f[4], f[5]), Pair16<T>::round(f[6], f[7]));
   }
 };
+template <typename T> struct Run<T, 1> {
+  using Raw = T;
+  using Raw8 = uint8_t;
+  static __device__ __forceinline__ void values(const T &v, float (&f)[1]) { f[0] = Elem<T>::load(&v); }
+  static __device__ __forceinline__ void values8(uint8_t v, uint32_t byte, float (&f)[1]) { f[0] = within<T>(unpack2(v).x * scale_of(byte)); }
+  static __device__ __forceinline__ void store(T *p, const float (&f)[1]) { Elem<T>::store(p, f[0]); }
+};
 
-template <typename T, int V>
-__global__ void __launch_bounds__(THREADS) act_grad_kernel(const __grid_constant__ ActGrad a, int chunks) {
+// ACT, Z8: what z is, known when the kernel is compiled (-1: looked up for each value, for rows that take no vectors).
+template <typename T, int V, int ACT, bool Z8>
+__global__ void __launch_bounds__(THREADS, 3) act_grad_kernel(const __grid_constant__ ActGrad a, int chunks) {
+  constexpr int DEEP = 4;      // rows whose loads are in flight together
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = (blockIdx.x * 32 + lane) * V;
   const long long r0 = a.rows * blockIdx.y / chunks, r1 = a.rows * (blockIdx.y + 1) / chunks;
   const unsigned n_blk = (unsigned)((a.cols + BLOCK - 1) / BLOCK);
+  const int kind = ACT < 0 ? a.act : ACT;
+  const bool z8 = ACT < 0 ? a.z8 != nullptr : Z8;
   float sum[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) sum[j] = 0.f;
+  grid_start();
   if (c < a.cols) {
-#pragma unroll 2
-    for (long long r = r0 + ty; r < r1; r += ROWS) {
-      float g[V], z[V];
-      Run<T, V>::load((const T *)a.gy + r * a.gy_stride + c, g);
-      if (a.z8) {
-        const float s = scale_of(a.z8_scale[r * n_blk + c / BLOCK]);
-        const uint8_t *src = a.z8 + r * a.cols + c;
-        if constexpr (V == 8) {
-          const uint2 v = *reinterpret_cast<const uint2 *>(src);
-          const uint32_t w[4] = {v.x & 0xFFFFu, v.x >> 16, v.y & 0xFFFFu, v.y >> 16};
+    for (long long r = r0 + ty; r < r1; r += ROWS * DEEP) {
+      typename Run<T, V>::Raw g_raw[DEEP], z_raw[DEEP];
+      typename Run<T, V>::Raw8 q_raw[DEEP];
+      uint32_t byte[DEEP];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float2 t = unpack2(w[j]);
-            z[2 * j] = within<T>(t.x * s);
-            z[2 * j + 1] = within<T>(t.y * s);
-          }
-        } else z[0] = within<T>(unpack2(*src).x * s);
-      } else if (a.z) Run<T, V>::load((const T *)a.z + r * a.z_stride + c, z);
-      if (a.act != WINOCONV_ACT_NONE) {
-#pragma unroll
-        for (int j = 0; j < V; ++j) g[j] *= act::slope(z[j], a.act);
+      for (int u = 0; u < DEEP; ++u) {
+        const long long at = r + u * ROWS;
+        if (at >= r1) break;
+        g_raw[u] = *reinterpret_cast<const typename Run<T, V>::Raw *>((const T *)a.gy + at * a.gy_stride + c);
+        if (kind != WINOCONV_ACT_NONE) {
+          if (z8) {
+            q_raw[u] = *reinterpret_cast<const typename Run<T, V>::Raw8 *>(a.z8 + at * a.cols + c);
+            byte[u] = a.z8_scale[at * n_blk + c / BLOCK];
+          } else z_raw[u] = *reinterpret_cast<const typename Run<T, V>::Raw *>((const T *)a.z + at * a.z_stride + c);
+        }
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += g[j];
-      if (a.dz) Run<T, V>::store((T *)a.dz + r * a.dz_stride + c, g);
+      for (int u = 0; u < DEEP; ++u) {
+        const long long at = r + u * ROWS;
+        if (at >= r1) break;
+        float g[V], z[V];
+        Run<T, V>::values(g_raw[u], g);
+        if (kind != WINOCONV_ACT_NONE) {
+          if (z8) Run<T, V>::values8(q_raw[u], byte[u], z);
+          else Run<T, V>::values(z_raw[u], z);
+#pragma unroll
+          for (int j = 0; j < V; ++j) g[j] *= act::slope(z[j], kind);
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] += g[j];
+        if (a.dz) Run<T, V>::store((T *)a.dz + at * a.dz_stride + c, g);
+      }
     }
   }
   if (!a.dbias) return;
@@ -245,6 +321,7 @@ __global__ void __launch_bounds__(THREADS) column_sum_kernel(const float *__rest
   __shared__ float part[ROWS][32];
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
+  grid_start();
   if (c < cols)
     for (int i = ty; i < chunks; i += ROWS) s += ws[(long long)i * cols + c];
   part[ty][lane] = s;
@@ -257,47 +334,61 @@ __global__ void __launch_bounds__(THREADS) column_sum_kernel(const float *__rest
 }
 
 bool on16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+bool on8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 unsigned blocks_of(unsigned long long n, unsigned per) { return (unsigned)((n + per - 1) / per); }
+
+template <typename... P, typename... A> cudaError_t launch(void (*kern)(P...), dim3 grid, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid; cfg.blockDim = dim3(THREADS); cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
 
 template <typename T>
 cudaError_t pack(const void *x, long long x_stride, long long rows, int cols, uint8_t *q, uint8_t *scale, cudaStream_t s) {
   const unsigned n_blk = (unsigned)((cols + BLOCK - 1) / BLOCK);
-  if (cols % 8 == 0 && on16(x) && x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0) {
-    const unsigned long long n = (unsigned long long)rows * n_blk * 4;
-    pack_kernel<T><<<blocks_of(n, THREADS * UNROLL), THREADS, 0, s>>>((const T *)x, x_stride, q, scale, n, n_blk * 4, cols);
-  } else {
-    const unsigned long long n = (unsigned long long)rows * n_blk;
-    pack_ragged_kernel<T><<<blocks_of(n, THREADS / 32 * UNROLL), THREADS, 0, s>>>((const T *)x, x_stride, q, scale, n, n_blk, cols);
+  const unsigned long long n = (unsigned long long)rows * n_blk;
+  if (cols % 8 == 0 && on16(x) && x_stride % 8 == 0 && on8(q)) {
+    const bool flat = cols % BLOCK == 0 && (x_stride == cols || rows == 1);
+    return launch(flat ? pack_kernel<T, true> : pack_kernel<T, false>, blocks_of(n * 4, THREADS * UNROLL), s, (const T *)x, x_stride, q, scale, n * 4, n_blk * 4, cols);
   }
-  return cudaGetLastError();
+  return launch(pack_ragged_kernel<T>, blocks_of(n, THREADS / 32 * UNROLL), s, (const T *)x, x_stride, q, scale, n, n_blk, cols);
 }
 template <typename T>
 cudaError_t unpack(const uint8_t *q, const uint8_t *scale, long long rows, int cols, void *x, long long x_stride, cudaStream_t s) {
   const unsigned n_blk = (unsigned)((cols + BLOCK - 1) / BLOCK);
-  if (cols % 8 == 0 && on16(x) && x_stride % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 7u) == 0) {
-    const unsigned long long n = (unsigned long long)rows * n_blk * 4;
-    unpack_kernel<T><<<blocks_of(n, THREADS * UNROLL), THREADS, 0, s>>>(q, scale, (T *)x, x_stride, n, n_blk * 4, cols);
-  } else {
-    const unsigned long long n = (unsigned long long)rows * n_blk;
-    unpack_ragged_kernel<T><<<blocks_of(n, THREADS / 32 * UNROLL), THREADS, 0, s>>>(q, scale, (T *)x, x_stride, n, n_blk, cols);
+  const unsigned long long n = (unsigned long long)rows * n_blk;
+  if (cols % 8 == 0 && on16(x) && x_stride % 8 == 0 && on8(q)) {
+    const bool flat = cols % BLOCK == 0 && (x_stride == cols || rows == 1);
+    return launch(flat ? unpack_kernel<T, true> : unpack_kernel<T, false>, blocks_of(n * 4, THREADS * UNROLL), s, q, scale, (T *)x, x_stride, n * 4, n_blk * 4, cols);
   }
-  return cudaGetLastError();
+  return launch(unpack_ragged_kernel<T>, blocks_of(n, THREADS / 32 * UNROLL), s, q, scale, (T *)x, x_stride, n, n_blk, cols);
 }
 
+template <typename T, int ACT> auto act_grad_kernel_of(bool z8) { return z8 ? act_grad_kernel<T, 8, ACT, true> : act_grad_kernel<T, 8, ACT, false>; }
 template <typename T> cudaError_t act_grad(const ActGrad &a, cudaStream_t s) {
-  const bool wide = a.cols % 8 == 0 && on16(a.gy) && a.gy_stride % 8 == 0 && (!a.z || (on16(a.z) && a.z_stride % 8 == 0)) &&
-                    (!a.z8 || (reinterpret_cast<uintptr_t>(a.z8) & 7u) == 0) && (!a.dz || (on16(a.dz) && a.dz_stride % 8 == 0));
+  const bool wide = a.cols % 8 == 0 && on16(a.gy) && a.gy_stride % 8 == 0 && (!a.z || (on16(a.z) && a.z_stride % 8 == 0)) && (!a.z8 || on8(a.z8)) &&
+                    (!a.dz || (on16(a.dz) && a.dz_stride % 8 == 0));
   const int chunks = act_grad_chunks(a.rows, a.cols), v = wide ? 8 : 1;
-  const dim3 grid((unsigned)((a.cols + 32 * v - 1) / (32 * v)), (unsigned)chunks);
-  if (wide) act_grad_kernel<T, 8><<<grid, THREADS, 0, s>>>(a, chunks);
-  else act_grad_kernel<T, 1><<<grid, THREADS, 0, s>>>(a, chunks);
-  const cudaError_t e = cudaGetLastError();
+  auto kern = act_grad_kernel<T, 1, -1, false>;
+  if (wide) {
+    switch (a.act) {
+      case WINOCONV_ACT_RELU: kern = act_grad_kernel_of<T, WINOCONV_ACT_RELU>(a.z8); break;
+      case WINOCONV_ACT_GELU: kern = act_grad_kernel_of<T, WINOCONV_ACT_GELU>(a.z8); break;
+      case WINOCONV_ACT_GELU_TANH: kern = act_grad_kernel_of<T, WINOCONV_ACT_GELU_TANH>(a.z8); break;
+      case WINOCONV_ACT_SILU: kern = act_grad_kernel_of<T, WINOCONV_ACT_SILU>(a.z8); break;
+      default: kern = act_grad_kernel<T, 8, WINOCONV_ACT_NONE, false>;
+    }
+  }
+  const cudaError_t e = launch(kern, dim3((unsigned)((a.cols + 32 * v - 1) / (32 * v)), (unsigned)chunks), s, a, chunks);
   if (e != cudaSuccess || !a.dbias) return e;
   const unsigned n = (unsigned)((a.cols + 31) / 32);
-  if (a.dbias_dtype == WINOCONV_F32) column_sum_kernel<float><<<n, THREADS, 0, s>>>(a.ws, (float *)a.dbias, a.cols, chunks);
-  else if (a.dbias_dtype == WINOCONV_F16) column_sum_kernel<__half><<<n, THREADS, 0, s>>>(a.ws, (__half *)a.dbias, a.cols, chunks);
-  else column_sum_kernel<__nv_bfloat16><<<n, THREADS, 0, s>>>(a.ws, (__nv_bfloat16 *)a.dbias, a.cols, chunks);
-  return cudaGetLastError();
+  if (a.dbias_dtype == WINOCONV_F32) return launch(column_sum_kernel<float>, n, s, a.ws, (float *)a.dbias, a.cols, chunks);
+  if (a.dbias_dtype == WINOCONV_F16) return launch(column_sum_kernel<__half>, n, s, a.ws, (__half *)a.dbias, a.cols, chunks);
+  return launch(column_sum_kernel<__nv_bfloat16>, n, s, a.ws, (__nv_bfloat16 *)a.dbias, a.cols, chunks);
 }
 
 }  // namespace e4m3
@@ -313,13 +404,12 @@ cudaError_t launch_e4m3_unpack(int dtype, const uint8_t *q, const uint8_t *scale
 cudaError_t launch_pad_rows(const void *x, long long x_stride, void *y, long long out_stride, long long rows, int cols, cudaStream_t s) {
   const unsigned per = (unsigned)(out_stride / 2);
   const unsigned long long n = (unsigned long long)rows * per;
-  pad_rows_kernel<<<blocks_of(n, THREADS * UNROLL), THREADS, 0, s>>>((const uint16_t *)x, x_stride, (uint16_t *)y, out_stride, n, per, cols);
-  return cudaGetLastError();
+  return launch(pad_rows_kernel, blocks_of(n, THREADS * UNROLL), s, (const uint16_t *)x, x_stride, (uint16_t *)y, out_stride, n, per, cols);
 }
-// Runs of rows: enough blocks for four on every SM, at least 32 rows to a run (so that the partial sums stay a few per cent of
+// Runs of rows: enough blocks for three on every SM, at least 32 rows to a run (so that the partial sums stay a few per cent of
 // what is read), at most 65535.
 int act_grad_chunks(long long rows, int cols) {
-  const long long strips = (cols + 255) / 256, want = std::max<long long>(1, (4LL * 148 + strips - 1) / strips);
+  const long long strips = (cols + 255) / 256, want = std::max<long long>(1, (3LL * 148 + strips - 1) / strips);
   return (int)std::max<long long>(1, std::min({want, (rows + 31) / 32, 65535LL}));
 }
 cudaError_t launch_act_grad(const ActGrad &a, cudaStream_t s) {
