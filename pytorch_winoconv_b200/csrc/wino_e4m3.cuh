@@ -64,67 +64,80 @@ template <typename T> __device__ __forceinline__ float within(float v) {      //
 namespace act {
 
 // The smooth activations are built from the hardware's 2^x and 1/x (each good to a few 2^-23 relative), far below the 2^-9 or
-// 2^-12 that rounding a result to 16 bits costs: a kernel that passes over memory has about 30 instructions a value to spend.
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+// 2^-12 that rounding a result to 16 bits costs, and work on two values an instruction: a kernel that passes over memory at
+// 6.5 TB/s has about 20 instructions a value to spend.
+struct F2 {      // two fp32 values
+  uint64_t v;
+  F2() = default;
+  __device__ __forceinline__ F2(uint64_t x) : v(x) {}
+  __device__ __forceinline__ F2(float a, float b) : v(f2_pack(a, b)) {}
+  __device__ __forceinline__ F2(float a) : v(f2_pack(a, a)) {}
+  __device__ __forceinline__ float lo() const { float a, b; f2_unpack(v, a, b); return a; }
+  __device__ __forceinline__ float hi() const { float a, b; f2_unpack(v, a, b); return b; }
+};
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) { return F2(f2_add(a.v, b.v)); }
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) { return F2(f2_mul(a.v, b.v)); }
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) { return F2(f2_fma(a.v, b.v, c.v)); }
+template <typename Op> __device__ __forceinline__ F2 each(F2 a, Op op) { return F2(op(a.lo()), op(a.hi())); }
+
+__device__ __forceinline__ F2 exp2_fast(F2 x) {
+  return each(x, [](float t) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t)); return y; });
 }
-__device__ __forceinline__ float recip(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
+__device__ __forceinline__ F2 recip(F2 x) {
+  return each(x, [](float t) { float y; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(t)); return y; });
 }
 constexpr float LOG2E = 1.4426950408889634f;
 // sqrt(2 / pi) and the cubic term of the tanh form of GELU; (1 + tanh u) / 2 = sigmoid(2 u)
 constexpr float GELU_C = 0.7978845608028654f, GELU_A = 0.044715f;
 
-__device__ __forceinline__ float sigmoid(float t) { return recip(1.f + exp2_fast(-LOG2E * t)); }
-__device__ __forceinline__ float clamp16(float z) {      // NaN passes
-  float y;
-  asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, 0f41800000;\n\tmax.NaN.f32 %0, t, 0fC1800000;\n\t}" : "=f"(y) : "f"(z));
-  return y;
-}
-// sigmoid(2 u) of the tanh form; z within +-16, beyond which it is 0 or 1 in fp32.
-__device__ __forceinline__ float gelu_sigmoid(float z, float z2) {
-  return recip(1.f + exp2_fast(z * fmaf(z2, -2.f * LOG2E * GELU_C * GELU_A, -2.f * LOG2E * GELU_C)));
+__device__ __forceinline__ F2 sigmoid(F2 t) { return recip(exp2_fast(t * F2(-LOG2E)) + F2(1.f)); }
+// sigmoid(2 u) of the tanh form.  z2: z squared, at most 256: sigmoid is 0 or 1 in fp32 from |z| = 16 on, and nothing overflows.
+__device__ __forceinline__ F2 square256(F2 z) { return each(z * z, [](float t) { return fminf(t, 256.f); }); }
+__device__ __forceinline__ F2 gelu_sigmoid(F2 z, F2 z2) {
+  return recip(exp2_fast(z * fma2(z2, F2(-2.f * LOG2E * GELU_C * GELU_A), F2(-2.f * LOG2E * GELU_C))) + F2(1.f));
 }
 // The normal distribution's integral, and its density, with one exponential: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with
 // t = 1 / (1 + p x) for x >= 0 (Abramowitz and Stegun, formula 7.1.26: within 1.5e-7 of erf).
-__device__ __forceinline__ float normal(float z, float &density) {
-  const float x = fabsf(z) * 0.7071067811865476f, e = exp2_fast(-LOG2E * x * x), t = recip(fmaf(0.3275911f, x, 1.f));
-  const float p = t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  const float tail = 0.5f * p * e;
-  density = 0.3989422804014327f * e;
-  return z < 0.f ? tail : 1.f - tail;
+__device__ __forceinline__ F2 normal(F2 z, F2 &density) {
+  const F2 x = each(z * F2(0.7071067811865476f), [](float t) { return fabsf(t); });
+  const F2 e = exp2_fast(x * x * F2(-LOG2E)), t = recip(fma2(x, F2(0.3275911f), F2(1.f)));
+  F2 p = fma2(t, F2(1.061405429f), F2(-1.453152027f));
+  p = fma2(t, p, F2(1.421413741f));
+  p = fma2(t, p, F2(-0.284496736f));
+  p = fma2(t, p, F2(0.254829592f));
+  const F2 tail = p * t * (e * F2(0.5f)), body = fma2(tail, F2(-1.f), F2(1.f));
+  density = e * F2(0.3989422804014327f);
+  return F2(z.lo() < 0.f ? tail.lo() : body.lo(), z.hi() < 0.f ? tail.hi() : body.hi());
 }
 
-__device__ __forceinline__ float apply(float z, int act) {
+__device__ __forceinline__ F2 apply(F2 z, int act) {
   switch (act) {
-    case WINOCONV_ACT_RELU: return z < 0.f ? 0.f : z;      // NaN passes
-    case WINOCONV_ACT_GELU: { float d; return z * normal(z, d); }
-    case WINOCONV_ACT_GELU_TANH: { const float c = clamp16(z); return z * gelu_sigmoid(c, c * c); }
+    case WINOCONV_ACT_RELU: return each(z, [](float t) { return t < 0.f ? 0.f : t; });      // NaN passes
+    case WINOCONV_ACT_GELU: { F2 d(0.f); return z * normal(z, d); }
+    case WINOCONV_ACT_GELU_TANH: return z * gelu_sigmoid(z, square256(z));
     case WINOCONV_ACT_SILU: return z * sigmoid(z);
     default: return z;
   }
 }
-__device__ __forceinline__ float slope(float z, int act) {
+// (products that could be 0 x infinity for large z are taken in the order that keeps them 0)
+__device__ __forceinline__ F2 slope(F2 z, int act) {
   switch (act) {
-    case WINOCONV_ACT_RELU: return z > 0.f ? 1.f : z <= 0.f ? 0.f : z;
+    case WINOCONV_ACT_RELU: return each(z, [](float t) { return t > 0.f ? 1.f : t <= 0.f ? 0.f : t; });
     case WINOCONV_ACT_GELU: {
-      float d;
-      const float c = clamp16(z), n = normal(c, d);      // the density is 0 beyond
-      return fmaf(c, d, n);
+      F2 d(0.f);
+      const F2 n = normal(z, d);
+      return fma2(z, d, n);
     }
     case WINOCONV_ACT_GELU_TANH: {
-      const float c = clamp16(z), c2 = c * c, s = gelu_sigmoid(c, c2);
-      return fmaf(c * fmaf(c2, 6.f * GELU_C * GELU_A, 2.f * GELU_C), fmaf(-s, s, s), s);
+      const F2 z2 = square256(z), s = gelu_sigmoid(z, z2);
+      const F2 h = fma2(s * F2(-1.f), s, s) * z;
+      return fma2(h, fma2(z2, F2(6.f * GELU_C * GELU_A), F2(2.f * GELU_C)), s);
     }
     case WINOCONV_ACT_SILU: {
-      const float s = sigmoid(z);
-      return fmaf(z * s, 1.f - s, s);
+      const F2 s = sigmoid(z);
+      return fma2(z * s, fma2(s, F2(-1.f), F2(1.f)), s);
     }
-    default: return 1.f;
+    default: return F2(1.f);
   }
 }
 

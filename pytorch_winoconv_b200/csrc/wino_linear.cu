@@ -116,7 +116,10 @@ __device__ __forceinline__ void finish4(const Out &o, int row, int col, float (&
       }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = act::apply(v[j], o.act);
+    for (int j = 0; j < 4; j += 2) {
+      const act::F2 y = act::apply(act::F2(v[j], v[j + 1]), o.act);
+      v[j] = y.lo(); v[j + 1] = y.hi();
+    }
     if (o.residual) {
       const T *src = (const T *)o.residual + row * o.residual_stride + col;
       float r[4] = {0.f, 0.f, 0.f, 0.f};
@@ -532,7 +535,10 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
             if (lane < rows) o.z8_scale[(long long)(row0 + lane) * n_blk + c / e4m3::BLOCK] = (uint8_t)byte;
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) f[i] = act::apply(f[i], ACT);
+          for (int i = 0; i < 32; i += 2) {
+            const act::F2 y = act::apply(act::F2(f[i], f[i + 1]), ACT);
+            f[i] = y.lo(); f[i + 1] = y.hi();
+          }
           if (o.residual) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
