@@ -261,7 +261,8 @@ WINOCONV_API int winoconv_backward_weight(const winoconv_desc_t *desc, const voi
  * matrices that the tensor cores read (x, w, dz) start on 16 bytes and have strides that are multiples of 8
  * (winoconv_pad_rows makes such a copy); the others may lie anywhere.  No scratch but where it is said.
  *   forward     z = x W^T + bias; y = act(z) + residual.  bias, residual may be NULL.  z (dtype) or z8 with z8_scale (eight bits,
- *               as winoconv_e4m3_pack writes them) receive the pre-activation where they are not NULL.
+ *               as winoconv_e4m3_pack writes them) receive the pre-activation where they are not NULL.  With one or two rows and
+ *               no z8, x and w may lie anywhere too.
  *   activation  dz = gy act'(z), dbias = sums of its columns.  z or z8 with z8_scale as kept by the forward (neither with
  *               WINOCONV_ACT_NONE); dz, dbias may be NULL; ws: winoconv_linear_backward_ws bytes where dbias is not NULL.
  *   data        dx = dz W.
@@ -294,8 +295,19 @@ WINOCONV_API int winoconv_linear_backward_data(const winoconv_linear_desc_t *des
                                                int64_t dx_stride, void *stream);
 WINOCONV_API int winoconv_linear_backward_weight(const winoconv_linear_desc_t *desc, const void *dz, int64_t dz_stride, const void *x, void *dw,
                                                  int dw_dtype, void *stream);
-/* x [rows][cols] of 16-bit values -> y [rows][y_stride] (a multiple of 8, y on 16 bytes), zeros from column `cols` on. */
-WINOCONV_API int winoconv_pad_rows(const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int32_t cols, void *stream);
+/*
+ * Copies of one or two matrices as the tensor cores read them, by one launch: x [rows][cols] in in_dtype (dtype or F32, rounded once) ->
+ * y [rows][y_stride] in dtype (F16 or BF16; y on 16 bytes, y_stride a multiple of 8), zeros from column `cols` on.
+ */
+typedef struct winoconv_rows {
+  const void *x;
+  int64_t x_stride;           /* elements; 0: no gap */
+  void *y;
+  int64_t y_stride;
+  int64_t rows;
+  int32_t cols, in_dtype, dtype, reserved;
+} winoconv_rows_t;
+WINOCONV_API int winoconv_pad_rows(const winoconv_rows_t *matrices, int32_t count, void *stream);
 
 /*
  * Activations kept in eight bits: 32 neighbours of a row share a power of two 2^e, the smallest (from 2^-127 on) that brings the

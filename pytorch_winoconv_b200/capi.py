@@ -59,6 +59,11 @@ class LinearDesc(Structure):
                 ("residual_stride", c_int64), ("y_stride", c_int64), ("z_stride", c_int64)]
 
 
+class Rows(Structure):
+    _fields_ = [("x", c_void_p), ("x_stride", c_int64), ("y", c_void_p), ("y_stride", c_int64), ("rows", c_int64), ("cols", c_int32),
+                ("in_dtype", c_int32), ("dtype", c_int32), ("reserved", c_int32)]
+
+
 class WinoconvError(RuntimeError):
     def __init__(self, status: int, what: str, detail: str):
         self.status = status
@@ -106,7 +111,7 @@ def lib() -> ctypes.CDLL:
                                                       c_int64, c_void_p, c_int, c_void_p, c_size_t, c_void_p]
     L.winoconv_linear_backward_data.argtypes = [POINTER(LinearDesc), c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p]
     L.winoconv_linear_backward_weight.argtypes = [POINTER(LinearDesc), c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p]
-    L.winoconv_pad_rows.argtypes = [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_void_p]
+    L.winoconv_pad_rows.argtypes = [POINTER(Rows), c_int32, c_void_p]
     L.winoconv_e4m3_pack.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p]
     L.winoconv_e4m3_unpack.argtypes = [c_int, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]
     for name in ("winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation",

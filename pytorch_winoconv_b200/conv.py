@@ -25,7 +25,9 @@ Backward (the reference left only traces of one: ``include/splitstrideone/split_
   filter, ``grad_x = conv(grad_y, flip(w)^T)`` with padding ``k - 1 - p`` (a stride-2 layer first spreads ``grad_y`` onto the
   stride grid), the weight gradient by one tensor-core GEMM per filter tap (``winoconv_gemm_batched``), the bias gradient a sum.
 
-A fused ReLU is differentiated through the stored output; the fused max-pool is forward only.
+A fused ReLU is differentiated through the stored output; the fused max-pool is forward only.  With ``checkpoint="e4m3"`` a 16-bit
+layer keeps its input in eight bits (and the ReLU as a byte for each value) instead of the tensors themselves: half the memory, the
+result and the data gradient unchanged, the weight gradient that of an input rounded to four significant bits.
 ``groups != 1`` and dilation raise (the reference accepts ``groups`` and silently computes groups = 1).
 """
 from __future__ import annotations
@@ -53,7 +55,7 @@ class _WinoConvMixin:
     _nd: int = 2
     MAX_CACHED_PLANS = 8      # distinct input shapes (and backward shapes) kept per module; the oldest is dropped
 
-    def _init_wino(self, compute_dtype, activation, pool, tile_m, algo):
+    def _init_wino(self, compute_dtype, activation, pool, tile_m, algo, checkpoint):
         if activation not in (None, "relu"):
             raise ValueError("activation must be None or 'relu'")
         if pool not in (None, 1, 2):
@@ -64,6 +66,11 @@ class _WinoConvMixin:
             raise NotImplementedError("groups != 1 is not supported (the reference ignores the argument)")
         if self.padding_mode != "zeros" or isinstance(self.padding, str):
             raise NotImplementedError("only explicit zero padding")
+        if checkpoint not in (None, "e4m3"):
+            raise ValueError("checkpoint must be None or 'e4m3'")
+        if checkpoint and compute_dtype == torch.float32:
+            raise NotImplementedError("checkpoint='e4m3' is for layers that compute in float16 or bfloat16")
+        self.checkpoint = checkpoint
         self.compute_dtype = compute_dtype
         self.activation = activation
         self.pool = 2 if pool == 2 else None
@@ -75,7 +82,7 @@ class _WinoConvMixin:
     # The forward and the autograd node are native (csrc/conv_module.cpp): plan lookup, filter transform, layout, allocation
     # and launch cost about 6 us a call where the same steps in Python cost 24.  What it does not take (an argument to
     # refuse, fp32 gradients) returns None and runs below.
-    _CONFIG = frozenset(("compute_dtype", "activation", "pool", "tile_m", "algo", "stride", "padding"))
+    _CONFIG = frozenset(("compute_dtype", "activation", "pool", "tile_m", "algo", "stride", "padding", "checkpoint"))
 
     def __call__(self, *args, **kwargs):
         """``torch.nn.Module.__call__`` without its 5 us of dispatch where there is no hook, tracer, compiled call or
@@ -108,13 +115,14 @@ class _WinoConvMixin:
 
     def __setstate__(self, state):
         super().__setstate__(state)
+        self.__dict__.setdefault("checkpoint", None)      # a module pickled before it had one
         self._reset_plans()
 
     def _make_runner(self):
         code = -1 if self.compute_dtype is None else engine.dtype_code(self.compute_dtype)
         self.__dict__["_runner"] = _backend.load().ConvRunner(
             self._nd, [int(s) for s in self.stride], [int(p) for p in self.padding], self.tile_m, self.algo,
-            self.activation == "relu", self.pool == 2, code, self.MAX_CACHED_PLANS)
+            self.activation == "relu", self.pool == 2, code, self.MAX_CACHED_PLANS, self.checkpoint is not None)
         return self._runner
 
     @property
@@ -175,6 +183,8 @@ class _WinoConvMixin:
             if self.pool:
                 raise NotImplementedError("the fused max-pool is forward only: use pool=None and a separate "
                                           "torch.nn.MaxPool2d where a gradient is needed")
+            if self.checkpoint:
+                raise NotImplementedError("checkpoint='e4m3' needs the native gradients: float16 or bfloat16, at most 400 taps")
             return _WinoConvFn.apply(self, input, self.weight, self.bias)
         return self._forward_no_grad(input)
 
@@ -270,6 +280,8 @@ class _WinoConvMixin:
             s += f", activation={self.activation}"
         if self.pool:
             s += f", pool={self.pool}"
+        if self.checkpoint:
+            s += f", checkpoint={self.checkpoint}"
         return s
 
     @property
@@ -318,7 +330,8 @@ class Conv2d(_WinoConvMixin, nn.Conv2d):
 
     Extra keyword arguments: ``compute_dtype`` (default ``torch.float16`` as upstream, ``None`` keeps the
     input's dtype; fp32 runs its products as three tf32 tensor-core products of a hi / lo split), ``activation`` (``None`` / ``"relu"``),
-    ``pool`` (``None`` / ``2``), ``tile_m`` (0 auto, 1 direct taps, 2, 4; 6 for fp32 layers) and ``algo`` (``capi.ALGO_*``).
+    ``pool`` (``None`` / ``2``), ``tile_m`` (0 auto, 1 direct taps, 2, 4; 6 for fp32 layers), ``algo`` (``capi.ALGO_*``) and
+    ``checkpoint`` (``None`` / ``"e4m3"``: what the gradients need of the input is kept in eight bits, :mod:`.checkpoint`).
     """
 
     _nd = 2
@@ -326,10 +339,10 @@ class Conv2d(_WinoConvMixin, nn.Conv2d):
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, groups=1, bias=True,
                  padding_mode="zeros", device=None, dtype=None, *, compute_dtype: Optional[torch.dtype] = torch.float16,
                  activation: Optional[str] = None, pool: Optional[int] = None, tile_m: int = 0,
-                 algo: int = capi.ALGO_AUTO):
+                 algo: int = capi.ALGO_AUTO, checkpoint: Optional[str] = None):
         nn.Conv2d.__init__(self, in_channels, out_channels, kernel_size, stride, padding, dilation, groups, bias,
                            padding_mode, device=device, dtype=dtype)
-        self._init_wino(compute_dtype, activation, pool, tile_m, algo)
+        self._init_wino(compute_dtype, activation, pool, tile_m, algo, checkpoint)
 
 
 class Conv3d(_WinoConvMixin, nn.Conv3d):
@@ -341,9 +354,9 @@ class Conv3d(_WinoConvMixin, nn.Conv3d):
     def __init__(self, in_channels, out_channels, kernel_size, stride=1, padding=0, dilation=1, groups=1, bias=True,
                  padding_mode="zeros", device=None, dtype=None, *, compute_dtype: Optional[torch.dtype] = torch.float16,
                  activation: Optional[str] = None, pool: Optional[int] = None, tile_m: int = 0,
-                 algo: int = capi.ALGO_AUTO):
+                 algo: int = capi.ALGO_AUTO, checkpoint: Optional[str] = None):
         if pool == 2:
             raise ValueError("pool=2 is the 2-D epilogue max-pool: not available on Conv3d")
         nn.Conv3d.__init__(self, in_channels, out_channels, kernel_size, stride, padding, dilation, groups, bias,
                            padding_mode, device=device, dtype=dtype)
-        self._init_wino(compute_dtype, activation, pool, tile_m, algo)
+        self._init_wino(compute_dtype, activation, pool, tile_m, algo, checkpoint)

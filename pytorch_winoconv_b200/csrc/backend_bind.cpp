@@ -28,7 +28,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return e4m3_unpack(q, scale, type);
   });
   py::class_<ConvRunner, c10::intrusive_ptr<ConvRunner>>(m, "ConvRunner")
-      .def(py::init<int64_t, std::vector<int64_t>, std::vector<int64_t>, int64_t, int64_t, bool, bool, int64_t, int64_t>())
+      .def(py::init<int64_t, std::vector<int64_t>, std::vector<int64_t>, int64_t, int64_t, bool, bool, int64_t, int64_t, bool>())
       .def("forward", &ConvRunner::forward, py::call_guard<py::gil_scoped_release>())
       .def("entries", [](ConvRunner &r) {
         py::list out;

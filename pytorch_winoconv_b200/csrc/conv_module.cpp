@@ -1,4 +1,5 @@
 #include "conv_module.h"
+#include "linear_module.h"
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -105,16 +106,23 @@ unsigned long long capture_of(cudaStream_t stream) {
 struct ConvFn : public torch::autograd::Function<ConvFn> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const c10::intrusive_ptr<ConvRunner> &runner, const at::Tensor &x,
                             const at::Tensor &x_cl, const std::shared_ptr<ConvRunner::Entry> &entry, const at::Tensor &weight,
-                            const std::optional<at::Tensor> &bias, bool relu) {
+                            const std::optional<at::Tensor> &bias, bool relu, bool pack) {
     at::Tensor y = runner->run(*entry, x_cl, weight, bias, weight.requires_grad());
-    ctx->save_for_backward({x, relu ? y : at::Tensor()});
+    if (pack) {      // x in eight bits where the weight gradient reads it, the ReLU as a byte for each value
+      at::AutoDispatchBelowADInplaceOrView no_graph;
+      at::Tensor q, scale;
+      if (weight.requires_grad()) std::tie(q, scale) = e4m3_pack(x_cl.movedim(1, -1));
+      ctx->save_for_backward({q, scale, relu ? y > 0 : at::Tensor()});
+      ctx->saved_data["x_sizes"] = x.sizes().vec();
+      ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
+    } else ctx->save_for_backward({x, relu ? y : at::Tensor()});
     ctx->saved_data["runner"] = c10::IValue::make_capsule(runner);
     ctx->saved_data["weight"] = weight;
     if (bias) ctx->saved_data["bias"] = *bias;
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-    torch::autograd::variable_list out(7);
+    torch::autograd::variable_list out(8);
     if (!grads[0].defined()) return out;
     auto saved = ctx->get_saved_variables();
     auto runner = c10::static_intrusive_pointer_cast<ConvRunner>(ctx->saved_data["runner"].toCapsule());
@@ -124,7 +132,17 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
     if (b != ctx->saved_data.end()) bias = b->second.toTensor();
     // numbered by the tensors among the arguments of apply: x, x_cl, weight, bias
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(2), nb = bias && ctx->needs_input_grad(3);
-    auto g = runner->backward(grads[0], saved[0], saved[1], weight, bias, nx, nw, nb);
+    std::vector<at::Tensor> g;
+    if (saved.size() == 3) {
+      at::AutoDispatchBelowADInplaceOrView no_graph;
+      c10::cuda::CUDAGuard guard(grads[0].device());
+      const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();
+      // (without the weight gradient nothing reads x: a tensor of its sizes stands for it)
+      const at::Tensor x = saved[0].defined() ? e4m3_unpack(saved[0], saved[1], runner->type_for(x_type)).movedim(-1, 1)
+                                              : at::empty({1}, grads[0].options().dtype(x_type)).expand(ctx->saved_data["x_sizes"].toIntVector());
+      g = runner->backward(saved[2].defined() ? grads[0] * saved[2].to(grads[0].scalar_type()) : grads[0], x, at::Tensor(), weight, bias, nx, nw && saved[0].defined(), nb);
+      if (g[0].defined() && g[0].scalar_type() != x_type) g[0] = g[0].to(x_type);
+    } else g = runner->backward(grads[0], saved[0], saved[1], weight, bias, nx, nw, nb);
     out[1] = g[0];
     out[4] = g[1];
     out[5] = g[2];
@@ -135,8 +153,8 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
 }  // namespace
 
 ConvRunner::ConvRunner(int64_t nd, std::vector<int64_t> stride, std::vector<int64_t> padding, int64_t tile_m, int64_t algo, bool relu,
-                       bool pool, int64_t compute, int64_t max_plans)
-    : nd_((int)nd), tile_m_((int)tile_m), algo_((int)algo), compute_((int)compute), relu_(relu), pool_(pool), max_plans_((size_t)max_plans) {
+                       bool pool, int64_t compute, int64_t max_plans, bool pack)
+    : nd_((int)nd), tile_m_((int)tile_m), algo_((int)algo), compute_((int)compute), relu_(relu), pool_(pool), pack_(pack), max_plans_((size_t)max_plans) {
   TORCH_CHECK((nd == 2 || nd == 3) && (int64_t)stride.size() == nd && (int64_t)padding.size() == nd, "ConvRunner: bad rank");
   for (int i = 0; i < 3; ++i) { stride_[i] = 1; pad_[i] = 0; }
   for (int i = 0; i < nd; ++i) { stride_[3 - nd + i] = (int)stride[i]; pad_[3 - nd + i] = (int)padding[i]; }
@@ -276,8 +294,10 @@ std::optional<at::Tensor> ConvRunner::forward(const at::Tensor &x, const at::Ten
     x_cl = dense_channels_last(x, type_of(dtype), stream_of());
     if (x_cl.is_same(x)) x_cl = x.detach();
   }
-  return ConvFn::apply(c10::intrusive_ptr<ConvRunner>::reclaim_copy(this), x, x_cl, e, weight, bias, relu_);
+  return ConvFn::apply(c10::intrusive_ptr<ConvRunner>::reclaim_copy(this), x, x_cl, e, weight, bias, relu_, pack_);
 }
+
+at::ScalarType ConvRunner::type_for(at::ScalarType x) const { return compute_ >= 0 ? type_of(compute_) : x; }
 
 void ConvRunner::Written::on(const c10::cuda::CUDAStream &here) {
   stream = here;

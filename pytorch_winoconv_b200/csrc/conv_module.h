@@ -27,7 +27,7 @@ std::optional<at::Tensor> conv_call(const at::Tensor &x, const at::Tensor &weigh
 class ConvRunner : public torch::CustomClassHolder {
  public:
   ConvRunner(int64_t nd, std::vector<int64_t> stride, std::vector<int64_t> padding, int64_t tile_m, int64_t algo, bool relu, bool pool,
-             int64_t compute, int64_t max_plans);
+             int64_t compute, int64_t max_plans, bool pack);      // pack: what the gradients need of x is kept in eight bits
 
   // The module's forward, or nothing where the Python path has to decide (an error to raise, a gradient the kernels do not cover).
   std::optional<at::Tensor> forward(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, bool training);
@@ -82,13 +82,14 @@ class ConvRunner : public torch::CustomClassHolder {
   // Gradients of one layer call; undefined where not asked for.
   std::vector<at::Tensor> backward(const at::Tensor &gy, const at::Tensor &x, const at::Tensor &y, const at::Tensor &weight,
                                    const std::optional<at::Tensor> &bias, bool need_x, bool need_w, bool need_b);
+  at::ScalarType type_for(at::ScalarType x) const;      // of operands and result for such an input
 
  private:
   std::shared_ptr<Entry> entry_for(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, int dtype, bool first);
   bool backward_covered(Entry &e);      // whether the native gradients take the layer
 
   int nd_, stride_[3], pad_[3], tile_m_, algo_, compute_;
-  bool relu_, pool_;
+  bool relu_, pool_, pack_;
   size_t max_plans_;
   std::mutex mu_;
   std::vector<std::shared_ptr<Entry>> entries_;     // most recently used last

@@ -37,29 +37,69 @@ int64_t row_stride(const at::Tensor &t) {
 }
 // A matrix with contiguous rows.
 at::Tensor with_rows(const at::Tensor &t) { return row_stride(t) ? t : t.contiguous(); }
-// A matrix as the tensor cores' loads want it: rows on 16 bytes.  Else a copy with padded rows (of which the first cols are seen).
-at::Tensor operand(const at::Tensor &in) {
-  const at::Tensor t = with_rows(in);
-  if (row_stride(t) % 8 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0) return t;
-  const int64_t rows = t.size(0), cols = t.size(1), ld = round8(cols);
-  at::Tensor out = at::empty({rows, ld}, plain(t));
-  check_abi(winoconv_pad_rows(t.data_ptr(), rows == 1 ? cols : row_stride(t), out.data_ptr(), ld, rows, (int32_t)cols, stream_of()), "winoconv_pad_rows");
-  return out.narrow(1, 0, cols);
-}
-// Its stride for the C ABI.
-int64_t ld_of(const at::Tensor &t) { return row_stride(t); }
+bool on16(const at::Tensor &t) { return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0; }
 
-at::Tensor as_rows(const at::Tensor &t, int64_t cols) { return t.reshape({-1, cols}); }
+at::Tensor as_rows(const at::Tensor &t, int64_t cols) { return t.dim() == 2 ? t : t.reshape({-1, cols}); }
 
-struct Shape {
-  int64_t rows, k, n;
+// A matrix as the C ABI takes it.
+struct Mat {
+  void *p = nullptr;
+  int64_t ld = 0;
 };
-winoconv_linear_desc_t describe(const Shape &s, at::ScalarType type, int act) {
+// The scratch of a call, allocated once, and the copies that its operands need, made by one launch: matrices whose rows do not
+// start on 16 bytes as the tensor cores' loads want them, and float weights, which are rounded.
+class Scratch {
+ public:
+  Scratch(int dtype, const at::Tensor &like) : dtype_(dtype), like_(like) {}
+  // The matrix itself, or a copy of it; `anywhere`: its rows need not start on 16 bytes.
+  void operand(const at::Tensor &in, Mat *m, bool anywhere = false) {
+    const at::Tensor t = with_rows(in);
+    const bool same = code_of(t.scalar_type()) == dtype_;
+    if (same && (anywhere || (row_stride(t) % 8 == 0 && on16(t)))) {
+      *m = {t.data_ptr(), row_stride(t)};
+    } else {
+      const int64_t rows = t.size(0), cols = t.size(1);
+      winoconv_rows_t &r = copies_[n_copies_];
+      r = {t.data_ptr(), rows == 1 ? 0 : row_stride(t), nullptr, round8(cols), rows, (int32_t)cols, code_of(t.scalar_type()), dtype_, 0};
+      at_[n_copies_] = take(rows * r.y_stride * 2);
+      to_[n_copies_++] = m;
+    }
+    alive_.push_back(t);
+  }
+  // Bytes for something else; pointer() of the result once allocate() has been called.
+  int64_t take(int64_t bytes) {
+    const int64_t at = bytes_;
+    bytes_ += (bytes + 255) / 256 * 256;
+    return at;
+  }
+  void allocate() {
+    if (bytes_ == 0) return;
+    buffer_ = at::empty({bytes_}, plain(like_).dtype(at::kByte));
+    for (int i = 0; i < n_copies_; ++i) {
+      copies_[i].y = pointer(at_[i]);
+      *to_[i] = {copies_[i].y, copies_[i].y_stride};
+    }
+    if (n_copies_ > 0) check_abi(winoconv_pad_rows(copies_, n_copies_, stream_of()), "winoconv_pad_rows");
+  }
+  void *pointer(int64_t at) const { return (uint8_t *)buffer_.data_ptr() + at; }
+
+ private:
+  int dtype_;
+  const at::Tensor &like_;
+  at::Tensor buffer_;
+  std::vector<at::Tensor> alive_;      // of views and copies that torch made
+  winoconv_rows_t copies_[2];
+  Mat *to_[2];
+  int64_t at_[2], bytes_ = 0;
+  int n_copies_ = 0;
+};
+
+winoconv_linear_desc_t describe(int64_t rows, int64_t k, int64_t n, at::ScalarType type, int act) {
   winoconv_linear_desc_t d = {};
-  TORCH_CHECK(s.rows <= 0x7fffffffLL && s.k <= 0x7fffffffLL && s.n <= 0x7fffffffLL, "linear: matrix too large");
-  d.rows = s.rows;
-  d.in_features = (int32_t)s.k;
-  d.out_features = (int32_t)s.n;
+  TORCH_CHECK(rows <= 0x7fffffffLL && k <= 0x7fffffffLL && n <= 0x7fffffffLL, "linear: matrix too large");
+  d.rows = rows;
+  d.in_features = (int32_t)k;
+  d.out_features = (int32_t)n;
   d.dtype = code_of(type);
   d.activation = act;
   return d;
@@ -74,33 +114,39 @@ at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tens
                    bool keep_z, Kept *kept) {
   const at::ScalarType type = x.scalar_type();
   const int64_t k = weight.size(1), n = weight.size(0);
-  at::Tensor x2 = as_rows(x, k);
-  const Shape s{x2.size(0), k, n};
-  std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
-  sizes.back() = n;
-  at::Tensor y = at::empty(sizes, plain(x));
+  const at::Tensor x2 = as_rows(x, k);
+  const int64_t rows = x2.size(0);
+  at::Tensor y;
+  if (x.dim() == 2) y = at::empty({rows, n}, plain(x));
+  else {
+    std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
+    sizes.back() = n;
+    y = at::empty(sizes, plain(x));
+  }
+  const bool z = kept && keep_z;
   if (kept && keep_x) {
     if (pack) std::tie(kept->x, kept->x_scale) = e4m3_pack(x2);
     else kept->x = x;
   }
-  if (kept && keep_z) {
-    if (pack) {
-      kept->z = at::empty({s.rows, n}, plain(x).dtype(at::kFloat8_e4m3fn));
-      kept->z_scale = at::empty({s.rows, (n + 31) / 32}, plain(x).dtype(at::kFloat8_e8m0fnu));
-    } else kept->z = at::empty({s.rows, n}, plain(x));
+  if (z) {
+    kept->z = at::empty({rows, n}, pack ? plain(x).dtype(at::kFloat8_e4m3fn) : plain(x));
+    if (pack) kept->z_scale = at::empty({rows, (n + 31) / 32}, plain(x).dtype(at::kFloat8_e8m0fnu));
   }
-  if (s.rows == 0) return y;
-  x2 = operand(x2);
-  const at::Tensor w = operand(weight.scalar_type() == type ? weight : weight.to(type));
+  if (rows == 0) return y;
+  winoconv_linear_desc_t d = describe(rows, k, n, type, act);
+  const bool anywhere = rows <= 2 && !(z && pack);      // one or two rows are read as they lie
+  Scratch scratch(d.dtype, x);
+  Mat xm, wm;
+  scratch.operand(x2, &xm, anywhere);
+  scratch.operand(weight, &wm, anywhere);
+  scratch.allocate();
   const at::Tensor b = bias.defined() ? bias.contiguous() : bias;
   const at::Tensor r = residual.defined() ? with_rows(as_rows(residual, n)) : residual;
-  winoconv_linear_desc_t d = describe(s, type, act);
   d.bias_f32 = b.defined() && b.scalar_type() == at::kFloat;
-  d.x_stride = ld_of(x2);
-  d.w_stride = ld_of(w);
-  if (r.defined() && s.rows > 1) d.residual_stride = ld_of(r);
-  const bool z = kept && keep_z;
-  check_abi(winoconv_linear_forward(&d, x2.data_ptr(), w.data_ptr(), b.defined() ? b.data_ptr() : nullptr, r.defined() ? r.data_ptr() : nullptr, y.data_ptr(),
+  d.x_stride = xm.ld;
+  d.w_stride = wm.ld;
+  if (r.defined() && rows > 1) d.residual_stride = row_stride(r);
+  check_abi(winoconv_linear_forward(&d, xm.p, wm.p, b.defined() ? b.data_ptr() : nullptr, r.defined() ? r.data_ptr() : nullptr, y.data_ptr(),
                                     z && !pack ? kept->z.data_ptr() : nullptr, z && pack ? kept->z.data_ptr() : nullptr,
                                     z && pack ? kept->z_scale.data_ptr() : nullptr, stream_of()),
             "winoconv_linear_forward");
@@ -108,6 +154,9 @@ at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tens
 }
 
 struct LinearFn : public torch::autograd::Function<LinearFn> {
+  // what the node remembers beside tensors, in one list of numbers: these, then the sizes of x
+  enum { X_TYPE, W_TYPE, B_TYPE, ACT, PACK, HAS_BIAS, HAS_RESIDUAL, OUT, IN, SIZES };
+
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias,
                             const std::optional<at::Tensor> &residual, int64_t act, bool pack) {
     const bool nx = x.requires_grad(), nw = weight.requires_grad(), nb = bias && bias->requires_grad();
@@ -119,10 +168,10 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
                     act != WINOCONV_ACT_NONE && (nx || nw || nb), &kept);
     }
     ctx->save_for_backward({kept.x, kept.x_scale, kept.z, kept.z_scale, nx ? weight : at::Tensor()});
-    ctx->saved_data["sizes"] = x.sizes().vec();
-    ctx->saved_data["w_sizes"] = weight.sizes().vec();
-    ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(), bias ? (int64_t)bias->scalar_type() : -1, act, pack};
-    ctx->saved_data["given"] = std::vector<int64_t>{bias.has_value(), residual.has_value()};
+    std::vector<int64_t> layer{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(), bias ? (int64_t)bias->scalar_type() : -1, act, pack,
+                               bias.has_value(), residual.has_value(), weight.size(0), weight.size(1)};
+    layer.insert(layer.end(), x.sizes().begin(), x.sizes().end());
+    ctx->saved_data["layer"] = std::move(layer);
     return y;
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
@@ -131,72 +180,71 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear: the gradients are not differentiable again (create_graph=True)");
     at::AutoDispatchBelowADInplaceOrView no_graph;
     const auto saved = ctx->get_saved_variables();
-    const auto sizes = ctx->saved_data["sizes"].toIntVector(), w_sizes = ctx->saved_data["w_sizes"].toIntVector(), types = ctx->saved_data["types"].toIntVector(),
-               given = ctx->saved_data["given"].toIntVector();
-    const auto type = (at::ScalarType)types[0], w_type = (at::ScalarType)types[1];
-    const int act = (int)types[3];
-    const bool pack = types[4] != 0;
+    const auto layer = ctx->saved_data["layer"].toIntVector();
+    const auto type = (at::ScalarType)layer[X_TYPE], w_type = (at::ScalarType)layer[W_TYPE];
+    const int act = (int)layer[ACT];
+    const bool pack = layer[PACK] != 0, slope = act != WINOCONV_ACT_NONE;
     // numbered by the tensors among the arguments of apply
-    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = given[0] && ctx->needs_input_grad(2),
-               nr = given[1] && ctx->needs_input_grad(2 + given[0]);
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = layer[HAS_BIAS] && ctx->needs_input_grad(2),
+               nr = layer[HAS_RESIDUAL] && ctx->needs_input_grad(2 + layer[HAS_BIAS]);
     const at::Tensor &gy = grads[0];
     c10::cuda::CUDAGuard guard(gy.device());
     if (nr) out[3] = gy;
     if (!nx && !nw && !nb) return out;
-    const int64_t n = w_sizes[0], k = w_sizes[1];
-    at::Tensor g = with_rows(as_rows(gy, n));
-    const Shape s{g.size(0), k, n};
+    const int64_t n = layer[OUT], k = layer[IN];
+    const at::Tensor g = with_rows(as_rows(gy, n));
+    const int64_t rows = g.size(0);
     at::Tensor dx, dw, db;
-    if (nw) dw = at::empty(w_sizes, plain(gy).dtype(w_type));
-    if (nb) db = at::empty({n}, plain(gy).dtype((at::ScalarType)types[2]));
-    if (nx) dx = at::empty(sizes, plain(gy));
-    if (s.rows == 0) {
-      if (nw) dw.zero_();
-      if (nb) db.zero_();
-    } else {
-      winoconv_linear_desc_t d = describe(s, type, act);
-      void *stream = stream_of();
-      const bool slope = act != WINOCONV_ACT_NONE;
-      // without an activation dz is gy as it lies, or a copy on 16 bytes
-      const bool copy = slope || ld_of(g) % 8 != 0 || (reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) != 0;
-      at::Tensor dz = g;
-      if (((nx || nw) && copy) || nb) {
-        at::Tensor ws;
-        uint64_t bytes = 0;
-        if (nb) {
-          check_abi(winoconv_linear_backward_ws(&d, &bytes), "winoconv_linear_backward_ws");
-          ws = at::empty({(int64_t)bytes}, plain(gy).dtype(at::kByte));
-        }
-        const bool write = (nx || nw) && copy;
-        if (write) dz = at::empty({s.rows, round8(n)}, plain(gy)).narrow(1, 0, n);
-        const bool z8 = slope && pack;
-        check_abi(winoconv_linear_backward_activation(&d, g.data_ptr(), s.rows > 1 ? ld_of(g) : 0, slope && !pack ? saved[2].data_ptr() : nullptr,
-                                                      z8 ? saved[2].data_ptr() : nullptr, z8 ? saved[3].data_ptr() : nullptr, write ? dz.data_ptr() : nullptr,
-                                                      write ? round8(n) : 0, nb ? db.data_ptr() : nullptr, nb ? code_of(db.scalar_type()) : 0,
-                                                      nb ? ws.data_ptr() : nullptr, bytes, stream),
-                  "winoconv_linear_backward_activation");
-      }
-      if (nx) {
-        const at::Tensor w = operand(saved[4].scalar_type() == type ? saved[4] : saved[4].to(type));
-        d.w_stride = ld_of(w);
-        check_abi(winoconv_linear_backward_data(&d, dz.data_ptr(), ld_of(dz), w.data_ptr(), dx.data_ptr(), 0, stream), "winoconv_linear_backward_data");
-      }
-      if (nw) {
-        at::Tensor x;
-        if (pack) {      // rows on 16 bytes
-          x = at::empty({s.rows, round8(k)}, plain(gy)).narrow(1, 0, k);
-          check_abi(winoconv_e4m3_unpack(d.dtype, saved[0].data_ptr(), saved[1].data_ptr(), s.rows, (int32_t)k, x.data_ptr(), round8(k), stream), "winoconv_e4m3_unpack");
-        } else x = operand(as_rows(saved[0], k));
-        d.x_stride = ld_of(x);
-        const bool direct = w_type == at::kFloat || w_type == type;
-        TORCH_CHECK(direct, "linear: weight type");
-        check_abi(winoconv_linear_backward_weight(&d, dz.data_ptr(), ld_of(dz), x.data_ptr(), dw.data_ptr(), code_of(w_type), stream),
-                  "winoconv_linear_backward_weight");
-      }
-    }
+    if (nw) dw = at::empty({n, k}, plain(gy).dtype(w_type));
+    if (nb) db = at::empty({n}, plain(gy).dtype((at::ScalarType)layer[B_TYPE]));
+    if (nx) dx = at::empty(at::IntArrayRef(layer.data() + SIZES, layer.size() - SIZES), plain(gy));
     out[0] = dx;
     out[1] = dw;
     out[2] = db;
+    if (rows == 0) {
+      if (nw) dw.zero_();
+      if (nb) db.zero_();
+      return out;
+    }
+    winoconv_linear_desc_t d = describe(rows, k, n, type, act);
+    void *stream = stream_of();
+    Scratch scratch(d.dtype, gy);
+    Mat dz{g.data_ptr(), row_stride(g)}, w, x;
+    // without an activation dz is gy as it lies, or a copy on 16 bytes
+    const bool write = (nx || nw) && (slope || dz.ld % 8 != 0 || !on16(g));
+    int64_t dz_at = 0, ws_at = 0, x_at = 0;
+    uint64_t ws_bytes = 0;
+    if (write) dz_at = scratch.take(rows * round8(n) * 2);
+    if (nb) {
+      check_abi(winoconv_linear_backward_ws(&d, &ws_bytes), "winoconv_linear_backward_ws");
+      ws_at = scratch.take((int64_t)ws_bytes);
+    }
+    if (nx) scratch.operand(saved[4], &w);
+    if (nw) {
+      if (pack) x_at = scratch.take(rows * round8(k) * 2);
+      else scratch.operand(as_rows(saved[0], k), &x);
+    }
+    scratch.allocate();
+    if (write || nb) {
+      if (write) dz = {scratch.pointer(dz_at), round8(n)};
+      check_abi(winoconv_linear_backward_activation(&d, g.data_ptr(), rows > 1 ? row_stride(g) : 0, slope && !pack ? saved[2].data_ptr() : nullptr,
+                                                    slope && pack ? saved[2].data_ptr() : nullptr, slope && pack ? saved[3].data_ptr() : nullptr,
+                                                    write ? dz.p : nullptr, write ? dz.ld : 0, nb ? db.data_ptr() : nullptr, nb ? code_of(db.scalar_type()) : 0,
+                                                    nb ? scratch.pointer(ws_at) : nullptr, ws_bytes, stream),
+                "winoconv_linear_backward_activation");
+    }
+    if (nx) {
+      d.w_stride = w.ld;
+      check_abi(winoconv_linear_backward_data(&d, dz.p, dz.ld, w.p, dx.data_ptr(), 0, stream), "winoconv_linear_backward_data");
+    }
+    if (nw) {
+      if (pack) {
+        x = {scratch.pointer(x_at), round8(k)};
+        check_abi(winoconv_e4m3_unpack(d.dtype, saved[0].data_ptr(), saved[1].data_ptr(), rows, (int32_t)k, x.p, x.ld, stream), "winoconv_e4m3_unpack");
+      }
+      d.x_stride = x.ld;
+      check_abi(winoconv_linear_backward_weight(&d, dz.p, dz.ld, x.p, dw.data_ptr(), code_of(w_type), stream), "winoconv_linear_backward_weight");
+    }
     return out;
   }
 };

@@ -499,15 +499,14 @@ int winoconv_device_check(void) {
   // A thread that has launched nothing yet has no context, and without one the driver's tensor map encoder refuses: an autograd
   // thread, or a caller's new thread, may come here first.
   static thread_local int bound = -1;
-  if (bound != dev) {
-    e = cudaSetDevice(dev);
-    if (e != cudaSuccess) { cudaGetLastError(); return fail(WINOCONV_ERR_NO_DEVICE, std::string("cudaSetDevice: ") + cudaGetErrorString(e)); }
-    bound = dev;
-  }
+  if (bound == dev) return WINOCONV_OK;      // this thread has been here with this device
+  e = cudaSetDevice(dev);
+  if (e != cudaSuccess) { cudaGetLastError(); return fail(WINOCONV_ERR_NO_DEVICE, std::string("cudaSetDevice: ") + cudaGetErrorString(e)); }
   int major = 0;
   e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   if (e != cudaSuccess) { cudaGetLastError(); return fail(WINOCONV_ERR_NO_DEVICE, std::string("cudaDeviceGetAttribute: ") + cudaGetErrorString(e)); }
   if (major != 10) return fail(WINOCONV_ERR_NO_DEVICE, "the kernels are built for sm_100a only; current device has compute capability major " + std::to_string(major));
+  bound = dev;
   return WINOCONV_OK;
 }
 
@@ -897,8 +896,12 @@ int winoconv_linear_forward(const winoconv_linear_desc_t *desc, const void *x, c
                             void *z8, void *z8_scale, void *stream) {
   int st = check_linear(desc);
   if (st != WINOCONV_OK) return st;
-  if ((st = check_operand(x, or_dense(desc->x_stride, desc->in_features), desc->in_features, "x")) != WINOCONV_OK) return st;
-  if ((st = check_operand(w, or_dense(desc->w_stride, desc->in_features), desc->in_features, "w")) != WINOCONV_OK) return st;
+  if (linear_by_rows(desc->rows, 1, z8 != nullptr)) {
+    if (!x || !w) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null x or w");
+    if ((st = check_element(x, 2, "x")) != WINOCONV_OK || (st = check_element(w, 2, "w")) != WINOCONV_OK) return st;
+  } else if ((st = check_operand(x, or_dense(desc->x_stride, desc->in_features), desc->in_features, "x")) != WINOCONV_OK ||
+             (st = check_operand(w, or_dense(desc->w_stride, desc->in_features), desc->in_features, "w")) != WINOCONV_OK)
+    return st;
   if (!y) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null y");
   if (!z8 != !z8_scale) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "z8 and z8_scale go together");
   if (z8 && (reinterpret_cast<uintptr_t>(z8) & 15u)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "z8 must start on 16 bytes");
@@ -1003,15 +1006,25 @@ static int check_rows(int64_t rows, int64_t cols, int64_t stride) {
   return WINOCONV_OK;
 }
 
-int winoconv_pad_rows(const void *x, int64_t x_stride, void *y, int64_t y_stride, int64_t rows, int32_t cols, void *stream) {
-  if (!x || !y) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null tensor");
-  int st = check_rows(rows, cols, x_stride);
+int winoconv_pad_rows(const winoconv_rows_t *matrices, int32_t count, void *stream) {
+  if (!matrices) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null matrices");
+  if (count < 1 || count > 2) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "one or two matrices");
+  PadRows p = {};
+  p.count = count;
+  for (int i = 0; i < count; ++i) {
+    const winoconv_rows_t &m = matrices[i];
+    if (!m.x || !m.y) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null tensor");
+    int st = check_rows(m.rows, m.cols, m.x_stride);
+    if (st != WINOCONV_OK) return st;
+    if (!is16(m.dtype) || (m.in_dtype != m.dtype && m.in_dtype != WINOCONV_F32)) return fail(WINOCONV_ERR_UNSUPPORTED, "rows are copied from f32 or their own type to f16 or bf16");
+    if (m.y_stride < m.cols || m.y_stride % 8 != 0 || !aligned16(m.y)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "y starts on 16 bytes with a row stride that is a multiple of 8 and holds a row");
+    if (m.y_stride > 0x7fffffffLL - 1024) return fail(WINOCONV_ERR_UNSUPPORTED, "matrix too large");
+    if ((st = check_element(m.x, m.in_dtype == WINOCONV_F32 ? 4 : 2, "x")) != WINOCONV_OK) return st;
+    p.m[i] = {m.x, m.y, or_dense(m.x_stride, m.cols), m.y_stride, m.rows, m.cols, m.in_dtype, m.dtype};
+  }
+  const int st = winoconv_device_check();
   if (st != WINOCONV_OK) return st;
-  if (y_stride < cols || y_stride % 8 != 0 || !aligned16(y)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "y starts on 16 bytes with a row stride that is a multiple of 8 and holds a row");
-  if (y_stride > 0x7fffffffLL - 1024) return fail(WINOCONV_ERR_UNSUPPORTED, "matrix too large");
-  if ((st = check_element(x, 2, "x")) != WINOCONV_OK) return st;
-  if ((st = winoconv_device_check()) != WINOCONV_OK) return st;
-  const cudaError_t e = launch_pad_rows(x, or_dense(x_stride, cols), y, y_stride, rows, cols, (cudaStream_t)stream);
+  const cudaError_t e = launch_pad_rows(p, (cudaStream_t)stream);
   return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "row copy launch");
 }
 

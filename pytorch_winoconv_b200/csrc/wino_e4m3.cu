@@ -45,6 +45,7 @@ __device__ __forceinline__ bool place(unsigned long long i, unsigned long long n
   }
 }
 // The kernels start while the one before them ends (programmatic dependent launch): nothing is read or written before this.
+// (Their pointers are not declared restrict: the compiler may move a load that it takes for one of unchanging memory.)
 __device__ __forceinline__ void grid_start() {
   sm100::grid_launch_dependents();
   sm100::grid_dependency_wait();
@@ -52,7 +53,7 @@ __device__ __forceinline__ void grid_start() {
 
 // Items of eight values, four lanes to a block.
 template <typename T, bool FLAT>
-__global__ void __launch_bounds__(THREADS) pack_kernel(const T *__restrict__ x, long long x_stride, uint8_t *__restrict__ q, uint8_t *__restrict__ scale,
+__global__ void __launch_bounds__(THREADS) pack_kernel(const T *x, long long x_stride, uint8_t *q, uint8_t *scale,
                                                        unsigned long long n_items, unsigned per_row, int cols) {
   const unsigned long long i0 = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
   uint4 v[UNROLL];
@@ -104,8 +105,8 @@ __global__ void __launch_bounds__(THREADS) pack_kernel(const T *__restrict__ x, 
 
 // A warp to a block, for rows of any length and place.
 template <typename T>
-__global__ void __launch_bounds__(THREADS) pack_ragged_kernel(const T *__restrict__ x, long long x_stride, uint8_t *__restrict__ q,
-                                                              uint8_t *__restrict__ scale, unsigned long long n_blocks, unsigned per_row, int cols) {
+__global__ void __launch_bounds__(THREADS) pack_ragged_kernel(const T *x, long long x_stride, uint8_t *q,
+                                                              uint8_t *scale, unsigned long long n_blocks, unsigned per_row, int cols) {
   const int lane = threadIdx.x & 31;
   const unsigned long long b0 = (unsigned long long)blockIdx.x * (THREADS / 32 * UNROLL) + (threadIdx.x >> 5);
   float v[UNROLL];
@@ -142,7 +143,7 @@ template <typename T> __device__ __forceinline__ uint2 values4(uint32_t q, uint3
 }
 
 template <typename T, bool FLAT>
-__global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ scale, T *__restrict__ x,
+__global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *q, const uint8_t *scale, T *x,
                                                          long long x_stride, unsigned long long n_items, unsigned per_row, int cols) {
   const unsigned long long i0 = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x;
   uint2 v[UNROLL];
@@ -173,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) unpack_kernel(const uint8_t *__restri
 }
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *__restrict__ q, const uint8_t *__restrict__ scale, T *__restrict__ x,
+__global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *q, const uint8_t *scale, T *x,
                                                                 long long x_stride, unsigned long long n_blocks, unsigned per_row, int cols) {
   const int lane = threadIdx.x & 31;
   const unsigned long long b0 = (unsigned long long)blockIdx.x * (THREADS / 32 * UNROLL) + (threadIdx.x >> 5);
@@ -191,20 +192,41 @@ __global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *_
   }
 }
 
-// Rows copied with zeros behind them; T is any 16-bit type.
-__global__ void __launch_bounds__(THREADS) pad_rows_kernel(const uint16_t *__restrict__ x, long long x_stride, uint16_t *__restrict__ y, long long out_stride,
-                                                           unsigned long long n_items, unsigned per_row, int cols) {
+// Rows copied with zeros behind them, eight values a thread; the second matrix by blocks of its own.
+__global__ void __launch_bounds__(THREADS) pad_rows_kernel(const __grid_constant__ PadRows p) {
+  const auto &m = p.m[blockIdx.y];
+  const unsigned per_row = (unsigned)(m.y_stride / 8);
+  const unsigned long long n_items = (unsigned long long)m.rows * per_row;
   grid_start();
-#pragma unroll
-  for (int u = 0; u < UNROLL; ++u) {
-    const unsigned long long i = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x + u * THREADS;
-    if (i >= n_items) return;
+  for (unsigned long long i = (unsigned long long)blockIdx.x * THREADS + threadIdx.x; i < n_items; i += (unsigned long long)gridDim.x * THREADS) {
     long long row;
     unsigned at;
     split_index(i, per_row, row, at);
-    const uint16_t *src = x + row * x_stride + at * 2;
-    const uint32_t a = (int)(at * 2) < cols ? src[0] : 0u, b = (int)(at * 2 + 1) < cols ? src[1] : 0u;
-    *reinterpret_cast<uint32_t *>(y + row * out_stride + at * 2) = a | (b << 16);
+    const int c = (int)at * 8;
+    const long long from = row * m.x_stride + c;
+    uint32_t w[4];
+    if (m.in_dtype == WINOCONV_F32) {
+      const float *src = (const float *)m.x + from;
+      float f[8];
+      if (c + 8 <= m.cols && (reinterpret_cast<uintptr_t>(src) & 15u) == 0) {
+        const float4 a = reinterpret_cast<const float4 *>(src)[0], b = reinterpret_cast<const float4 *>(src)[1];
+        f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = c + j < m.cols ? src[j] : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        w[j] = m.dtype == WINOCONV_F16 ? Pair16<__half>::round(f[2 * j], f[2 * j + 1]) : Pair16<__nv_bfloat16>::round(f[2 * j], f[2 * j + 1]);
+    } else {
+      const uint16_t *src = (const uint16_t *)m.x + from;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a = c + 2 * j < m.cols ? src[2 * j] : 0u, b = c + 2 * j + 1 < m.cols ? src[2 * j + 1] : 0u;
+        w[j] = a | (b << 16);
+      }
+    }
+    *reinterpret_cast<uint4 *>((uint16_t *)m.y + row * m.y_stride + c) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
@@ -312,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, 4) act_grad_kernel(const __grid_const
 }
 
 template <typename O>
-__global__ void __launch_bounds__(THREADS) column_sum_kernel(const float *__restrict__ ws, O *__restrict__ out, int cols, int chunks) {
+__global__ void __launch_bounds__(THREADS) column_sum_kernel(const float *ws, O *out, int cols, int chunks) {
   __shared__ float part[ROWS][32];
   const int lane = threadIdx.x & 31, ty = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   float s = 0.f;
@@ -396,10 +418,10 @@ cudaError_t launch_e4m3_pack(int dtype, const void *x, long long x_stride, long 
 cudaError_t launch_e4m3_unpack(int dtype, const uint8_t *q, const uint8_t *scale, long long rows, int cols, void *x, long long x_stride, cudaStream_t s) {
   return dtype == WINOCONV_F16 ? unpack<__half>(q, scale, rows, cols, x, x_stride, s) : unpack<__nv_bfloat16>(q, scale, rows, cols, x, x_stride, s);
 }
-cudaError_t launch_pad_rows(const void *x, long long x_stride, void *y, long long out_stride, long long rows, int cols, cudaStream_t s) {
-  const unsigned per = (unsigned)(out_stride / 2);
-  const unsigned long long n = (unsigned long long)rows * per;
-  return launch(pad_rows_kernel, blocks_of(n, THREADS * UNROLL), s, (const uint16_t *)x, x_stride, (uint16_t *)y, out_stride, n, per, cols);
+cudaError_t launch_pad_rows(const PadRows &p, cudaStream_t s) {
+  unsigned long long n = 1;
+  for (int i = 0; i < p.count; ++i) n = std::max(n, (unsigned long long)p.m[i].rows * (unsigned long long)(p.m[i].y_stride / 8));
+  return launch(pad_rows_kernel, dim3((unsigned)std::min<unsigned long long>((n + THREADS - 1) / THREADS, 16 * 148), (unsigned)p.count), s, p);
 }
 // Runs of rows: multiples of the 32 that a block has in flight, short enough for three waves of four blocks on every SM (so that
 // the last wave costs little; the partial sums stay below a tenth of what is read), at most 65535 of them.

@@ -18,6 +18,7 @@
 // Roles: warp 0 TMA, warp 1 MMA issue; then all eight warps move the accumulator to shared memory and add up and store their share
 // of the rows.  Every mbarrier wait is bounded and reports through the error word.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 #include <set>
 #include <utility>
@@ -69,6 +70,15 @@ template <bool PAIR> __device__ __forceinline__ void load_operand(uint32_t dst, 
   if (!mn) load(dst, k, row);
   else
     for (int j = 0; j < n; j += 64) load(dst + (uint32_t)j * 128u, row + j, k);
+}
+// The same box on its way into L2.
+__device__ __forceinline__ void prefetch_operand(const CUtensorMap *map, int mn, int row, int n, int k) {
+  auto fetch = [&](int c0, int c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1) : "memory");
+  };
+  if (!mn) fetch(k, row);
+  else
+    for (int j = 0; j < n; j += 64) fetch(row + j, k);
 }
 // Low descriptor word of an operand tile and the step between its 16-value slices (16-byte units).  MN-major: blocks of 64 rows
 // 8 KB apart, groups of eight reduction steps 1 KB apart; K-major: groups of eight rows 1 KB apart.
@@ -159,6 +169,7 @@ struct ClusterArgs {
 };
 
 constexpr int CLUSTER_THREADS = 256;
+constexpr int CLUSTER_SMEM2 = 113 * 1024;      // of an SM's 228 KB for each of two CTAs, 1 KB of which is the system's
 
 template <typename T>
 __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
@@ -169,8 +180,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *base_ptr = smem_raw + (base - raw);
   const uint32_t stage_bytes = (uint32_t)(C_BYTES + g.tile_rows * BK * 2);
-  // the barriers lie behind the ring or the sums, whichever is longer
-  const uint32_t ring = max((uint32_t)g.stages * stage_bytes, (uint32_t)(g.tile_rows * BC * 4));
+  const uint32_t ring = max((uint32_t)g.stages * stage_bytes, (uint32_t)(g.tile_rows * BC * 4));      // or the sums, whichever is longer
   const uint32_t bars = base + ring;      // full[8] empty[8] done
   auto full = [&](int i) { return bars + 8u * i; };
   auto empty = [&](int i) { return bars + 64u + 8u * i; };
@@ -186,7 +196,10 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   uint32_t tmem_cols = 32;
   while (tmem_cols < (uint32_t)g.tile_rows) tmem_cols *= 2;
 
-  if (warp == 1 && lane == 0) { prefetch_map(&map_r); prefetch_map(&map_c); }
+  if (warp == 1 && lane == 0) prefetch_map(&map_r);
+  // The first stages of C (the weights) are sent for while this kernel sets itself up and the one before it ends; into L2 only,
+  // where the writes of the one before it would arrive too, should it be the one that changes them.
+  if (warp == 3 && lane < g.stages && k0 + lane < k1) prefetch_operand(&map_c, g.c_mn, col0, BC, (k0 + lane) * BK);
   if (warp == 0) {
     if (lane < 8) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
     else if (lane == 8) mbar_init(done, 1);
@@ -292,6 +305,122 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
     tc_fence_after();
     tmem_free<false>(tmem, tmem_cols);
   }
+}
+
+// ---- row kernel ------------------------------------------------------------------------------------------------------
+// One or two rows against weights that are read once: a block takes four rows of W and all of x, its threads eight neighbouring
+// values of the reduction each, twice before the first products; products by FMA (two values an instruction), and no set-up of
+// barriers and tensor memory.  Sums: a thread's own in the order of the reduction, then over the lanes, then over the warps.
+//
+// What bounds it is the read of W: one row of 4096 -> 16384 or 16384 -> 4096 (bf16) 20.7 us, 6.5 TB/s; 4096 -> 4096 7.2 us for 34 MB,
+// two of which are the launch (the cluster kernel: 24.0, 23.8 and 9.0 us).  Eight rows of W and one step, or no word to L2 ahead of
+// the kernel before: 9.6 and 7.5 us.  From three rows on the products cost more than the set-up (10.5 us against 8.6).
+constexpr int ROW_THREADS = 256, ROW_FEATURES = 4, MOST_ROWS = 2;
+
+// Lane sums of V values: afterwards v[0] of a lane is the sum over the warp of value `lane / (32 / V)`, with bits reversed as the
+// halving leaves them (index_of).
+template <int V> __device__ __forceinline__ void sum_lanes(float (&v)[V], int lane) {
+#pragma unroll
+  for (int n = V, d = 16; n > 1; n >>= 1, d >>= 1) {
+#pragma unroll
+    for (int i = 0; i < n / 2; ++i) {
+      const bool up = (lane & d) != 0;
+      const float keep = up ? v[i + n / 2] : v[i], send = up ? v[i] : v[i + n / 2];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+    }
+  }
+#pragma unroll
+  for (int d = 16 / V; d > 0; d >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+}
+
+template <typename T, int ROWS, bool WIDE>
+__global__ void __launch_bounds__(ROW_THREADS, 3) row_kernel(const T *x, long long x_stride, const T *w, long long w_stride, int red,
+                                                          const __grid_constant__ Out o) {
+  using act::F2;
+  constexpr int FEATURES = ROW_FEATURES, V = ROWS * FEATURES, WARPS = ROW_THREADS / 32;
+  static_assert(V <= 32, "a lane for every sum");
+  __shared__ float part[WARPS][V];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col0 = (int)blockIdx.x * FEATURES;
+  const T *wr[FEATURES];
+#pragma unroll
+  for (int f = 0; f < FEATURES; ++f) wr[f] = w + (long long)min(col0 + f, o.cols - 1) * w_stride;
+  if (WIDE) {      // the first steps' weights on their way to L2 while the kernel before this one ends
+    const int k = threadIdx.x * 64;
+    if (k < min(red, ROW_THREADS * 16))
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f) asm volatile("prefetch.global.L2 [%0];" ::"l"(wr[f] + k));
+  }
+  grid_launch_dependents();
+  grid_dependency_wait();
+  float v[V];
+  if constexpr (WIDE) {
+    F2 acc[ROWS][FEATURES];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f) acc[r][f] = F2(0.f);
+#pragma unroll 2
+    for (int k = threadIdx.x * 8; k < red; k += ROW_THREADS * 8) {
+      uint4 wv[FEATURES], xv[ROWS];
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f)
+        asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(wv[f].x), "=r"(wv[f].y), "=r"(wv[f].z), "=r"(wv[f].w) : "l"(wr[f] + k));
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) xv[r] = r < o.rows ? *reinterpret_cast<const uint4 *>(x + r * x_stride + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        F2 xs[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+          const float2 t = Pair16<T>::unpack(i == 0 ? xv[r].x : i == 1 ? xv[r].y : i == 2 ? xv[r].z : xv[r].w);
+          xs[r] = F2(t.x, t.y);
+        }
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) {
+          const float2 t = Pair16<T>::unpack(i == 0 ? wv[f].x : i == 1 ? wv[f].y : i == 2 ? wv[f].z : wv[f].w);
+          const F2 ws(t.x, t.y);
+#pragma unroll
+          for (int r = 0; r < ROWS; ++r) acc[r][f] = act::fma2(xs[r], ws, acc[r][f]);
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f) v[r * FEATURES + f] = acc[r][f].lo() + acc[r][f].hi();
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+#pragma unroll 2
+    for (int k = threadIdx.x; k < red; k += ROW_THREADS) {
+      float ws[FEATURES];
+#pragma unroll
+      for (int f = 0; f < FEATURES; ++f) ws[f] = Elem<T>::load(wr[f] + k);
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r) {
+        const float xs = r < o.rows ? Elem<T>::load(x + r * x_stride + k) : 0.f;
+#pragma unroll
+        for (int f = 0; f < FEATURES; ++f) v[r * FEATURES + f] = fmaf(xs, ws[f], v[r * FEATURES + f]);
+      }
+    }
+  }
+  sum_lanes<V>(v, lane);
+  // the value that the halving left here: its index has the lane's upper bits, first halving first
+  constexpr int LANES = 32 / V;
+  const int index = lane / LANES;
+  if (lane % LANES == 0) part[warp][index] = v[0];
+  __syncthreads();
+  if (threadIdx.x >= V) return;
+  float z = 0.f;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) z += part[i][threadIdx.x];
+  const int row = threadIdx.x / FEATURES, col = col0 + threadIdx.x % FEATURES;
+  if (row >= o.rows || col >= o.cols) return;
+  if (o.bias) z += o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[col] : Elem<T>::load((const T *)o.bias + col);
+  if (o.z) Elem<T>::store((T *)o.z + row * o.z_stride + col, z);
+  float y = act::apply(F2(z), o.act).lo();
+  if (o.residual) y += Elem<T>::load((const T *)o.residual + row * o.residual_stride + col);
+  Elem<T>::store((T *)o.y + row * o.y_stride + col, y);
 }
 
 // ---- pair kernel -----------------------------------------------------------------------------------------------------
@@ -651,8 +780,19 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
   return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 4), g, plan.split);
 }
 
-template <typename T, int ACT>
-cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+template <typename T> cudaError_t launch_rows(const LinearProblem &p, cudaStream_t s) {
+  const bool wide = p.red % 8 == 0 && multiple(p.r.ptr, p.r.stride, 2, 16) && multiple(p.c.ptr, p.c.stride, 2, 16);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((p.cols + ROW_FEATURES - 1) / ROW_FEATURES)); cfg.blockDim = dim3(ROW_THREADS); cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr; cfg.numAttrs = 1;
+  auto kern = p.rows == 1 ? (wide ? row_kernel<T, 1, true> : row_kernel<T, 1, false>) : (wide ? row_kernel<T, 2, true> : row_kernel<T, 2, false>);
+  return cudaLaunchKernelEx(&cfg, kern, (const T *)p.r.ptr, p.r.stride, (const T *)p.c.ptr, p.c.stride, p.red, out_of(p, 1));
+}
+
+template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
   CUtensorMap mr, mc;
   if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, 128) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, 128)) {
     *detail = "cuTensorMapEncodeTiled failed";
@@ -694,26 +834,49 @@ template <typename T> cudaError_t launch_pair(const LinearProblem &p, EncodeTile
 
 using namespace linear;
 
-// Tile and cluster of a problem: rows to a tile as many as there are, up to 128; then as many CTAs to a tile's reduction as
-// bring the grid nearest to two on every SM from below.
+bool linear_by_rows(long long rows, int layer, bool z8) { return layer && rows <= MOST_ROWS && !z8; }
+
+// The form with the smallest estimated time (us).  The constants are a fit to every form's time on 180 problems (B200, bf16: 3 to
+// 2048 rows, 500 to 16384 columns, reductions of 64 to 25088, the three placements of the operands; launches in a row, operands from
+// HBM): the form chosen takes 1.016 times the fastest one's time on geometric average and 1.15 times at worst.
 LinearPlan linear_plan(const LinearProblem &p) {
   LinearPlan plan = {};
-  const long long pair_tiles = (long long)((p.rows + PAIR_TILE - 1) / PAIR_TILE) * ((p.cols + PAIR_TILE - 1) / PAIR_TILE);
-  plan.pair = p.rows > 128 && pair_tiles >= 32;
-  if (plan.pair) return plan;
-  const int unit = p.r.mn ? 64 : 16;
-  plan.tile_rows = std::min(128, (p.rows + unit - 1) / unit * unit);
-  const long long tiles = (long long)((p.rows + plan.tile_rows - 1) / plan.tile_rows) * ((p.cols + BC - 1) / BC);
-  const int n_steps = (p.red + BK - 1) / BK;
-  plan.split = 1;
-  while (plan.split < 8 && tiles * plan.split * 2 <= 2LL * SMS && plan.split * 2 <= n_steps) plan.split *= 2;
-  const int budget = 113 * 1024 - 1024 - 1024 - BAR_BYTES;      // of an SM's 228 KB with 1 KB of the system's for each CTA
-  plan.stages = std::min(8, budget / (C_BYTES + plan.tile_rows * BK * 2));
+  plan.by_rows = linear_by_rows(p.rows, p.layer, p.z8 != nullptr);
+  if (plan.by_rows) return plan;
+  auto over = [](long long a, long long b) { return (a + b - 1) / b; };
+  const long long n_ct = over(p.cols, BC), n_steps = over(p.red, BK);
+  const double memory = 2.0 + 2.0 * ((double)p.rows * p.red + (double)p.cols * p.red + (double)p.rows * p.cols) / 6.2e6;
+  const double pair_waves = (double)over(over(p.rows, PAIR_TILE) * over(p.cols, PAIR_TILE), SMS / 2);
+  plan.pair = 1;
+  double best = std::max(memory, 4.11 + pair_waves * (0.36 * n_steps + 0.33));
+  for (int rows = p.r.mn ? 64 : 16; rows <= 256; rows *= 2) {
+    const long long n_rt = over(p.rows, rows);
+    if (rows < 256 && n_rt > 16) continue;                                   // many small tiles: never the fastest
+    for (int split = 1; split <= 8 && split <= n_steps; split *= 2)
+      for (int per_sm = 1; per_sm <= (rows == 256 ? 1 : 2); ++per_sm) {
+        // CTAs that are resident at a time: clusters do not fill every group of SMs
+        const int slots = per_sm * (split < 4 ? SMS : split == 4 ? (per_sm == 1 ? 132 : 142) : (per_sm == 1 ? 120 : 132));
+        const double ctas = (double)(n_rt * n_ct * split), full = ctas / slots, waves = full <= 3 ? std::ceil(full) : full + 0.5;
+        const double stage = C_BYTES + rows * BK * 2, shared = std::max(1.0, std::min(ctas, (double)slots) / SMS);
+        const double step = std::max(0.363, stage * shared * 9.5e-6);        // what a step waits for, or an SM's share of L2
+        const double end = 0.035 * rows + (split > 1 ? 1.2 : 0.0) + 0.28 * split;
+        const double t = std::max(memory, waves * ((double)over(n_steps, split) * step + end));
+        if (t < best) {
+          best = t;
+          plan.pair = 0;
+          plan.tile_rows = rows;
+          plan.split = split;
+          plan.stages = (int)std::min(8.0, ((per_sm == 1 ? 227 * 1024 : CLUSTER_SMEM2) - 1024 - BAR_BYTES) / stage);
+        }
+      }
+    if (rows >= p.rows) break;
+  }
   return plan;
 }
 
 cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
   *detail = "";
+  if (plan.by_rows) return p.dtype == WINOCONV_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
   if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, enc, s, detail) : launch_pair<__nv_bfloat16>(p, enc, s, detail);

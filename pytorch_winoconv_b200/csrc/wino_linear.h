@@ -28,16 +28,27 @@ struct LinearProblem {
 };
 // pair: a tile of 256 x 256 by two CTAs, tiles walked by a persistent grid.  Else a tile of `tile_rows` x 128 by a cluster of
 // `split` CTAs that share its reduction.
+// by_rows: a layer's few rows without the tensor cores.
 struct LinearPlan {
-  int pair;
+  int by_rows, pair;
   int tile_rows, split, stages;
 };
 LinearPlan linear_plan(const LinearProblem &p);
+bool linear_by_rows(long long rows, int layer, bool z8);      // such a problem's operands may lie anywhere
 cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail);
 cudaError_t read_and_clear_linear_error(cudaStream_t s, unsigned int *code);
 
-// Rows of `cols` 16-bit values copied to rows `out_stride` apart (a multiple of 8), zeros behind them.
-cudaError_t launch_pad_rows(const void *x, long long x_stride, void *y, long long out_stride, long long rows, int cols, cudaStream_t s);
+// One or two matrices copied to rows y_stride apart (a multiple of 8), zeros behind them; f32 rounded to dtype.
+struct PadRows {
+  struct {
+    const void *x;
+    void *y;
+    long long x_stride, y_stride, rows;
+    int cols, in_dtype, dtype;
+  } m[2];
+  int count;
+};
+cudaError_t launch_pad_rows(const PadRows &p, cudaStream_t s);
 
 // dz = gy * act'(z) and the sums of its columns.  z in dtype, or in 8 bits with its scales; dz may be null (act none), dbias too.
 struct ActGrad {

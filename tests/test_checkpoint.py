@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from pytorch_winoconv_b200 import capi, checkpoint
+from pytorch_winoconv_b200 import capi, checkpoint, conv
 from tests.test_linear import values8
 
 gpu = pytest.mark.gpu
@@ -118,6 +118,120 @@ def test_refusals_on_the_device():
                        (lambda: checkpoint.unpack(x, scale), "float8_e4m3fn"), (lambda: checkpoint.unpack(q, scale.cpu()), "same one")):
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+# ---- convolution layers that keep their input in eight bits ----------------------------------------------------------------
+LAYERS = [(conv.Conv2d, (2, 16, 9, 11), 24, 3, 1, 1, True), (conv.Conv2d, (3, 5, 14, 10), 8, 3, 2, 1, True), (conv.Conv2d, (2, 72, 12, 8), 40, 5, 1, 2, False),
+          (conv.Conv2d, (4, 64, 7, 7), 31, 1, 1, 0, True), (conv.Conv3d, (2, 8, 5, 6, 7), 16, 3, 1, 1, True)]
+
+
+def rounded(x):
+    """x as eight bits hold it, per pixel over the channels."""
+    return checkpoint.unpack(*checkpoint.pack(x.movedim(1, -1)), x.dtype).movedim(-1, 1)
+
+
+@gpu
+@pytest.mark.parametrize("cls,shape,k,ks,stride,pad,bias", LAYERS)
+@pytest.mark.parametrize("activation", [None, "relu"])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_convolution_layers(cls, shape, k, ks, stride, pad, bias, activation, dtype):
+    """Result, data and bias gradient are those of the layer without it, to the bit; the weight gradient is that of the rounded input."""
+    torch.manual_seed(3)
+    args, kw = (shape[1], k, ks), dict(stride=stride, padding=pad, bias=bias, compute_dtype=dtype)
+    plain = cls(*args, activation=activation, **kw).cuda()
+    kept = cls(*args, activation=activation, checkpoint="e4m3", **kw).cuda()
+    linear = cls(*args, **kw).cuda()
+    for m in (kept, linear):
+        m.load_state_dict(plain.state_dict())
+    x = torch.randn(shape, device="cuda").to(dtype).requires_grad_()
+
+    def run(m, t, gy=None):
+        y = m(t)
+        gy = torch.randn(y.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(dtype) if gy is None else gy
+        return y.detach(), gy, torch.autograd.grad(y, [t, *m.parameters()], gy)
+
+    y0, gy, g0 = run(plain, x)
+    y1, _, g1 = run(kept, x)
+    assert torch.equal(y0, y1) and torch.equal(g0[0], g1[0])
+    if bias:
+        assert torch.equal(g0[2], g1[2])
+    masked = gy * (y0 > 0).to(dtype) if activation else gy
+    _, _, g2 = run(linear, rounded(x.detach()).requires_grad_(), masked)
+    assert torch.equal(g1[1], g2[1])
+    assert not torch.equal(g1[1], g0[1])
+    assert capi.read_device_error() == 0
+
+
+@gpu
+def test_what_a_convolution_layer_keeps():
+    layer = conv.Conv2d(64, 32, 3, padding=1, activation="relu", checkpoint="e4m3").cuda()
+    x = torch.randn(4, 64, 20, 20, device="cuda", requires_grad=True)      # float input: kept as the rounded operand's eight bits
+    size = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: size.append(t.numel() * t.element_size()) or t, lambda t: t):
+        y = layer(x)
+    assert sorted(size) == sorted([x.numel(), x.numel() // 32, y.numel()])
+    y.float().sum().backward()
+    assert x.grad.dtype == torch.float32 and layer.weight.grad is not None
+    layer.weight.requires_grad_(False)
+    size.clear()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: size.append(t.numel() * t.element_size()) or t, lambda t: t):
+        y = layer(x)
+    assert size == [y.numel()]
+    plain = conv.Conv2d(64, 32, 3, padding=1, activation="relu").cuda()
+    plain.load_state_dict(layer.state_dict())
+    dx, db = torch.autograd.grad(y.float().sum(), (x, layer.bias))
+    dx2, db2 = torch.autograd.grad(plain(x).float().sum(), (x, plain.bias))
+    # (the bias gradient without the weight gradient beside it is another order of the same sum of ones)
+    assert torch.equal(dx, dx2) and torch.equal(db, db2)
+    assert layer.eval()(x).grad_fn is not None and "checkpoint=e4m3" in repr(layer)
+
+
+@gpu
+def test_a_convolution_and_a_linear_layer_in_a_captured_step():
+    """A small network as it would be trained, both layers keeping eight bits: the captured step gives the eager one's gradients."""
+    from pytorch_winoconv_b200 import linear
+    torch.manual_seed(0)
+    body = conv.Conv2d(8, 32, 3, padding=1, activation="relu", checkpoint="e4m3").cuda()
+    head = linear.Linear(32 * 36, 10, checkpoint="e4m3").cuda()
+    x = torch.randn(6, 8, 6, 6, device="cuda")
+    params = [*body.parameters(), *head.parameters()]
+
+    def step():
+        y = head(body(x).flatten(1))
+        return [y.detach(), *torch.autograd.grad(y.float().square().mean(), params)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    x.copy_(torch.randn(6, 8, 6, 6, device="cuda"))
+    with torch.no_grad():
+        for p in params:
+            p.mul_(0.5)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, step()))
+    assert capi.read_device_error() == 0
+
+
+@gpu
+def test_convolution_refusals_on_the_device():
+    layer = conv.Conv2d(4, 8, 3, compute_dtype=None, checkpoint="e4m3").cuda()
+    with pytest.raises(NotImplementedError, match="checkpoint"):
+        layer(torch.randn(1, 4, 8, 8, device="cuda", requires_grad=True))      # computes in float32
+    with torch.no_grad():
+        assert layer(torch.randn(1, 4, 8, 8, device="cuda")).shape == (1, 8, 6, 6)      # nothing to keep
+
+
+def test_convolution_refusals():
+    with pytest.raises(ValueError, match="checkpoint"):
+        conv.Conv2d(4, 8, 3, checkpoint="int8")
+    with pytest.raises(NotImplementedError, match="checkpoint"):
+        conv.Conv3d(4, 8, 3, compute_dtype=torch.float32, checkpoint="e4m3")
 
 
 def test_refusals_of_the_c_abi():

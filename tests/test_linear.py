@@ -60,7 +60,7 @@ def check(got, want, act, dtype, extra=None):
     assert (off <= tol).all(), ((off - tol).max().item(), off.max().item())
 
 
-SHAPES = [(1, 64, 128), (1, 1, 1), (1, 1000, 1531), (2, 33, 7), (3, 4096, 250), (16, 72, 136), (17, 129, 131), (31, 520, 2048), (64, 2048, 129),
+SHAPES = [(1, 64, 128), (1, 1, 1), (1, 1000, 1531), (1, 4103, 130), (2, 33, 7), (2, 4608, 1001), (3, 4096, 250), (16, 72, 136), (17, 129, 131), (31, 520, 2048), (64, 2048, 129),
           (127, 40, 64), (128, 64, 128), (129, 65, 129), (130, 777, 1000), (257, 200, 520), (1000, 136, 96), (1025, 100, 300), (513, 1024, 768),
           (1301, 72, 1531), (2000, 129, 1100), (1281, 1801, 1537), (1536, 1600, 1792)]
 
@@ -503,6 +503,10 @@ def test_refusals_of_the_c_abi():
                          (fwd(desc(), res=p + 1), bad), (fwd(desc(), z=p + 1), bad), (fwd(desc(), z8=p), bad), (fwd(desc(), zs=p), bad),
                          (fwd(desc(), z8=p + 8, zs=p), bad)):
         assert status == want, capi.last_error()
+    one = desc(rows=1)      # read as they lie, but for z8
+    for status, want in ((fwd(one, x=p + 1), bad), (fwd(one, w=p + 1), bad), (fwd(one, x=None), bad), (fwd(one, w=None), bad), (fwd(one, y=None), bad),
+                         (fwd(one, x=p + 2, z8=p, zs=p), bad)):
+        assert status == want, capi.last_error()
 
     def act(d, gy=p, gs=0, z=None, z8=None, zs=None, dz=p, dzs=0, db=None, dbt=0, ws=None, n=0):
         return lib.winoconv_linear_backward_activation(d, gy, gs, z, z8, zs, dz, dzs, db, dbt, ws, n, None)
@@ -521,10 +525,17 @@ def test_refusals_of_the_c_abi():
                          (weight(desc(), p, 0, p, None, 0, None), bad), (weight(desc(), p, 0, p, p, capi.BF16, None), unsupported),
                          (weight(desc(), p, 0, p + 4, p, 0, None), bad), (weight(desc(), p, 0, p, p + 2, 0, None), bad)):
         assert status == want, capi.last_error()
-    pad = lib.winoconv_pad_rows
-    for status, want in ((pad(None, 0, p, 8, 1, 8, None), bad), (pad(p, 0, p, 9, 1, 8, None), bad), (pad(p, 0, p, 8, 1, 9, None), bad), (pad(p, 0, p + 8, 8, 1, 8, None), bad),
-                         (pad(p, 4, p, 8, 1, 8, None), bad), (pad(p, 0, p, 8, 0, 8, None), bad), (pad(p + 1, 0, p, 8, 1, 8, None), bad)):
-        assert status == want, capi.last_error()
+    def pad(count=1, **kw):
+        m = (capi.Rows * 2)()
+        for i in range(2):
+            m[i] = capi.Rows(**{**dict(x=p, y=p, y_stride=8, rows=1, cols=8, in_dtype=capi.F16, dtype=capi.F16), **(kw if i == count - 1 else {})})
+        return lib.winoconv_pad_rows(m, count, None)
+
+    for count in (1, 2):
+        for kw, want in ((dict(x=None), bad), (dict(y=None), bad), (dict(y_stride=9), bad), (dict(cols=9), bad), (dict(y=p + 8), bad), (dict(x_stride=4), bad), (dict(rows=0), bad),
+                         (dict(x=p + 1), bad), (dict(x=p + 2, in_dtype=capi.F32), bad), (dict(in_dtype=capi.BF16), unsupported), (dict(dtype=capi.F32), unsupported)):
+            assert pad(count, **kw) == want, capi.last_error()
+    assert pad(0) == bad and pad(3) == bad and lib.winoconv_pad_rows(None, 1, None) == bad
 
 
 def test_the_c_abi_reports_a_missing_device():
