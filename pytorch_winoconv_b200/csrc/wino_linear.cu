@@ -80,86 +80,153 @@ __device__ __forceinline__ void prefetch_operand(const CUtensorMap *map, int mn,
   else
     for (int j = 0; j < n; j += 64) fetch(row + j, k);
 }
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
 // Low descriptor word of an operand tile and the step between its 16-value slices (16-byte units).  MN-major: blocks of 64 rows
 // 8 KB apart, groups of eight reduction steps 1 KB apart; K-major: groups of eight rows 1 KB apart.
 __device__ __forceinline__ uint32_t operand_lo(uint32_t saddr, int mn) { return desc_lo(saddr, mn ? 8192u : 16u); }
 __device__ __forceinline__ uint32_t operand_step(int mn) { return mn ? 128u : 2u; }
 
-// Four neighbouring columns of a row, summed: bias, activation, residual, and what is kept of z.
-template <typename T>
-__device__ __forceinline__ void finish4(const Out &o, int row, int col, float (&v)[4]) {
-  const bool any = col < o.cols;
+// A lane's four columns of a row in the cluster kernel's epilogue.  WIDE: neighbours, moved as one vector; else 32 apart, so that a
+// warp's accesses of single values are contiguous.
+template <bool WIDE> __device__ __forceinline__ int column_of(int lane, int j) { return WIDE ? 4 * lane + j : lane + 32 * j; }
+template <typename T, bool WIDE> __device__ __forceinline__ void load4(const T *row, int lane, int cols, float (&v)[4]) {
+  if constexpr (WIDE) {
+    if (4 * lane < cols) VecIO<T, 4>::load(row + 4 * lane, v);
+    else v[0] = v[1] = v[2] = v[3] = 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = lane + 32 * j < cols ? Elem<T>::load(row + lane + 32 * j) : 0.f;
+  }
+}
+template <typename T, bool WIDE> __device__ __forceinline__ void store4(T *row, int lane, int cols, const float (&v)[4]) {
+  if constexpr (WIDE) {
+    if (4 * lane < cols) VecIO<T, 4>::store(row + 4 * lane, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (lane + 32 * j < cols) Elem<T>::store(row + lane + 32 * j, v[j]);
+  }
+}
+// The sums v of a row's 128 columns from `col` on, finished and stored.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void finish4(const Out &o, int row, int col, int lane, float (&v)[4], const float (&bias)[4], const float (&residual)[4]) {
+  const int cols = o.cols - col;      // left of the matrix from here on
   if (o.layer) {
-    if (o.bias) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < o.cols) v[j] += o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[col + j] : Elem<T>::load((const T *)o.bias + col + j);
-    }
+    for (int j = 0; j < 4; ++j) v[j] += bias[j];
     if (o.z8) {      // (columns beyond the last are zero: no part in a block's scale)
-      float top = 0.f;
+      float top[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) top = fmaxf(top, e4m3::finite_magnitude(v[j]));
+      for (int j = 0; j < 4; ++j) top[j] = e4m3::finite_magnitude(v[j]);
+      if (WIDE) {    // a block is eight lanes' columns
+        float t = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
 #pragma unroll
-      for (int d = 1; d < 8; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-      const uint32_t byte = e4m3::scale_byte(top);
-      const float inv = e4m3::inverse_scale(byte);
-      const uint32_t q = e4m3::pack2(v[0], v[1], inv) | (e4m3::pack2(v[2], v[3], inv) << 16);
-      if (any) {
-        uint8_t *dst = o.z8 + (long long)row * o.cols + col;
-        if ((o.cols & 3) == 0) *reinterpret_cast<uint32_t *>(dst) = q;
-        else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (col + j < o.cols) dst[j] = (uint8_t)(q >> (8 * j));
-        }
-        if ((col & (e4m3::BLOCK - 1)) == 0) o.z8_scale[(long long)row * ((o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK) + col / e4m3::BLOCK] = (uint8_t)byte;
-      }
-    }
-    if (!any) return;
-    if (o.z) {
-      T *dst = (T *)o.z + row * o.z_stride + col;
-      if (o.wide) VecIO<T, 4>::store(dst, v);
-      else {
+        for (int d = 1; d < 8; d <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, d));
+        top[0] = top[1] = top[2] = top[3] = t;
+      } else {       // or one column of every lane
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (col + j < o.cols) Elem<T>::store(dst + j, v[j]);
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) top[j] = fmaxf(top[j], __shfl_xor_sync(0xffffffffu, top[j], d));
+      }
+      uint8_t *dst = o.z8 + (long long)row * o.cols + col, *scale = o.z8_scale + (long long)row * ((o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK) + col / e4m3::BLOCK;
+      if (WIDE) {
+        const uint32_t byte = e4m3::scale_byte(top[0]);
+        const float inv = e4m3::inverse_scale(byte);
+        if (4 * lane < cols) {
+          *reinterpret_cast<uint32_t *>(dst + 4 * lane) = e4m3::pack2(v[0], v[1], inv) | (e4m3::pack2(v[2], v[3], inv) << 16);
+          if ((lane & 7) == 0) scale[lane >> 3] = (uint8_t)byte;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t byte = e4m3::scale_byte(top[j]);
+          if (lane + 32 * j < cols) {
+            dst[lane + 32 * j] = (uint8_t)e4m3::pack2(v[j], 0.f, e4m3::inverse_scale(byte));
+            if (lane == 0) scale[j] = (uint8_t)byte;
+          }
+        }
       }
     }
+    if (o.z) store4<T, WIDE>((T *)o.z + row * o.z_stride + col, lane, cols, v);
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
       const act::F2 y = act::apply(act::F2(v[j], v[j + 1]), o.act);
-      v[j] = y.lo(); v[j + 1] = y.hi();
-    }
-    if (o.residual) {
-      const T *src = (const T *)o.residual + row * o.residual_stride + col;
-      float r[4] = {0.f, 0.f, 0.f, 0.f};
-      if (o.wide) VecIO<T, 4>::load(src, r);
-      else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < o.cols) r[j] = Elem<T>::load(src + j);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += r[j];
+      v[j] = y.lo() + residual[j]; v[j + 1] = y.hi() + residual[j + 1];
     }
   }
-  if (!any) return;
-  if (o.out_f32) {
-    float *dst = (float *)o.y + row * o.y_stride + col;
-    if (o.wide) VecIO<float, 4>::store(dst, v);
-    else {
+  if (o.out_f32) store4<float, WIDE>((float *)o.y + row * o.y_stride + col, lane, cols, v);
+  else store4<T, WIDE>((T *)o.y + row * o.y_stride + col, lane, cols, v);
+}
+
+// A warp's rows of a tile: j0, j0 + step, ... below n.  The bias and the residuals of the first PRE rows are loaded while the
+// products are still on their way.
+template <typename T, bool WIDE> struct RowEnd {
+  static constexpr int PRE = 4;
+  float bias[4] = {}, residual[PRE][4] = {};
+
+  __device__ __forceinline__ void load(const Out &o, int row0, int col, int lane, int j, float (&r)[4]) const {
+    load4<T, WIDE>((const T *)o.residual + (row0 + j) * o.residual_stride + col, lane, o.cols - col, r);
+  }
+  __device__ __forceinline__ void early(const Out &o, int row0, int col, int lane, int j0, int step, int n) {
+    if (!o.layer) return;
+    if (o.bias) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < o.cols) dst[j] = v[j];
+      for (int j = 0; j < 4; ++j) {
+        const int c = col + column_of<WIDE>(lane, j);
+        if (c < o.cols) bias[j] = o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[c] : Elem<T>::load((const T *)o.bias + c);
+      }
     }
-  } else {
-    T *dst = (T *)o.y + row * o.y_stride + col;
-    if (o.wide) VecIO<T, 4>::store(dst, v);
-    else {
+    if (o.residual) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (col + j < o.cols) Elem<T>::store(dst + j, v[j]);
+      for (int i = 0; i < PRE; ++i)
+        if (j0 + i * step < n) load(o, row0, col, lane, j0 + i * step, residual[i]);
     }
+  }
+  // sums(j, v): a lane's four columns of row j, added up over the parts of the reduction
+  template <typename Sums> __device__ __forceinline__ void run(const Out &o, int row0, int col, int lane, int j0, int step, int n, Sums &&sums) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < PRE; ++i) {
+      const int j = j0 + i * step;
+      if (j >= n) return;
+      sums(j, v);
+      finish4<T, WIDE>(o, row0 + j, col, lane, v, bias, residual[i]);
+    }
+#pragma unroll 1
+    for (int j = j0 + PRE * step; j < n; j += step) {
+      float r[4] = {0.f, 0.f, 0.f, 0.f};
+      if (o.residual) load(o, row0, col, lane, j, r);
+      sums(j, v);
+      finish4<T, WIDE>(o, row0 + j, col, lane, v, bias, r);
+    }
+  }
+};
+
+// A row's sums over the S CTAs of a cluster, from the same place in the shared memory of each: all parts' values in flight at once,
+// added in the same order by every CTA.
+template <int S, bool WIDE> __device__ __forceinline__ void add_parts(uint32_t sums, int j, int lane, float (&v)[4]) {
+  float u[S][4];
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    const uint32_t row = map_to_rank(sums + (uint32_t)((j * BC + (WIDE ? 4 * lane : lane)) * 4), (uint32_t)i);
+    if (WIDE) {
+      const float4 t = ld_cluster_f4(row);
+      u[i][0] = t.x; u[i][1] = t.y; u[i][2] = t.z; u[i][3] = t.w;
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) u[i][c] = ld_cluster_f1(row + 128u * c);
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    v[c] = u[0][c];
+#pragma unroll
+    for (int i = 1; i < S; ++i) v[c] += u[i][c];
   }
 }
 
@@ -171,7 +238,7 @@ struct ClusterArgs {
 constexpr int CLUSTER_THREADS = 256;
 constexpr int CLUSTER_SMEM2 = 113 * 1024;      // of an SM's 228 KB for each of two CTAs, 1 KB of which is the system's
 
-template <typename T>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
     cluster_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Out o,
                    const __grid_constant__ ClusterArgs g, int split) {
@@ -213,7 +280,6 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   uint32_t tmem;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
-  grid_launch_dependents();
   grid_dependency_wait();
 
   if (warp == 0) {
@@ -254,48 +320,39 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
     if (alive && elect_one()) umma_commit<false>(done, 0);
   }
   __syncwarp();
+  const int n = min(g.tile_rows, o.rows - row0);
+  RowEnd<T, WIDE> end;
+  end.early(o, row0, col0, lane, (int)part + warp * split, 8 * split, n);
   // sums to shared memory: [row][128 columns]
   const bool ok = mbar_wait_warp(done, 0, abort_word, err, ERR_DONE);
+  grid_launch_dependents();
   float *sums = reinterpret_cast<float *>(base_ptr);
   if (ok && *abort_word == 0u) {
     tc_fence_after();
     const int q = warp & 3;
-    for (int c = (warp >> 2) * 32; c < g.tile_rows; c += 64) {
+    for (int c = (warp >> 2) * 32; c < n; c += 64) {
       uint32_t v[32];
       tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
       tmem_wait_ld_x32(v);
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (c + j < g.tile_rows) sums[(c + j) * BC + q * 32 + lane] = __uint_as_float(v[j]);
+        if (c + j < n) sums[(c + j) * BC + q * 32 + lane] = __uint_as_float(v[j]);
     }
     tc_fence_before();
   }
   __syncthreads();
   if (split > 1) cluster_sync_all();
   if (*abort_word == 0u) {
-    const int n = min(g.tile_rows, o.rows - row0);
-    for (int j = (int)part + warp * split; j < n; j += 8 * split) {
-      float v[4];
-      const uint32_t src = base + (uint32_t)((j * BC + lane * 4) * 4);
+    end.run(o, row0, col0, lane, (int)part + warp * split, 8 * split, n, [&](int j, float (&v)[4]) {
       if (split == 1) {
-        const float4 u = *reinterpret_cast<const float4 *>(sums + j * BC + lane * 4);
-        v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-      } else {
-        auto add_parts = [&](auto n_parts) {      // all parts' values in flight at once, added in the same order by every CTA
-          constexpr int S = decltype(n_parts)::value;
-          float4 u[S];
 #pragma unroll
-          for (int i = 0; i < S; ++i) u[i] = ld_cluster_f4(map_to_rank(src, (uint32_t)i));
-          v[0] = u[0].x; v[1] = u[0].y; v[2] = u[0].z; v[3] = u[0].w;
-#pragma unroll
-          for (int i = 1; i < S; ++i) { v[0] += u[i].x; v[1] += u[i].y; v[2] += u[i].z; v[3] += u[i].w; }
-        };
-        if (split == 2) add_parts(std::integral_constant<int, 2>());
-        else if (split == 4) add_parts(std::integral_constant<int, 4>());
-        else add_parts(std::integral_constant<int, 8>());
+        for (int i = 0; i < 4; ++i) v[i] = sums[j * BC + column_of<WIDE>(lane, i)];
+        return;
       }
-      finish4<T>(o, row0 + j, col0 + lane * 4, v);
-    }
+      if (split == 2) add_parts<2, WIDE>(base, j, lane, v);
+      else if (split == 4) add_parts<4, WIDE>(base, j, lane, v);
+      else add_parts<8, WIDE>(base, j, lane, v);
+    });
   }
   __syncwarp();
   if (split > 1) cluster_sync_all();      // no CTA leaves while another reads its shared memory
@@ -759,7 +816,8 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
     *detail = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = cluster_kernel<T>;
+  const Out o = out_of(p, 4);
+  auto kern = o.wide ? cluster_kernel<T, true> : cluster_kernel<T, false>;
   cudaError_t e = allow_smem((const void *)kern);
   if (e != cudaSuccess) return e;
   ClusterArgs g;
@@ -777,7 +835,7 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = (unsigned)plan.split; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr; cfg.numAttrs = plan.split > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 4), g, plan.split);
+  return cudaLaunchKernelEx(&cfg, kern, mr, mc, o, g, plan.split);
 }
 
 template <typename T> cudaError_t launch_rows(const LinearProblem &p, cudaStream_t s) {
