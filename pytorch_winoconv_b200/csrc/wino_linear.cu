@@ -481,14 +481,23 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) row_kernel(const T *x, long lo
 }
 
 // ---- pair kernel -----------------------------------------------------------------------------------------------------
-constexpr int PAIR_THREADS = 384, PAIR_STAGES = 6;
-constexpr int PAIR_TILE = 256;                                    // rows and columns of a tile; a CTA holds half of each operand
-constexpr int PAIR_STAGE = 2 * 128 * BK * 2;                      // bytes a CTA loads for a stage
+// Many rows: a tile of 256 rows x BN columns by a CTA pair (cta_group::2, M = 256: each CTA loads half of both operands and holds
+// the sums of its 128 rows), a persistent grid, two accumulators so that eight epilogue warps finish a tile beside the next one's
+// products.  What bounds it: with 256 columns the tensor pipe under the power cap (8192 x 4096 x 16384 in bf16 0.65 ms in short runs,
+// 1690 TFLOP/s; 0.79 ms in long ones, where the library product takes 0.78); with 128 and 64, for problems of few tiles, the L2 (a step of
+// 64 takes 0.20 and 0.18 us where the pipe would take 0.14 and 0.07; four stages instead of eight 0.31, words to L2 ahead of the loads
+// only add to its work; 512 x 4096 x 4096 18.1 us with 128 columns, 26.3 with 256, 22.0 by the cluster kernel).
+constexpr int PAIR_THREADS = 384;
+constexpr int PAIR_ROWS = 256;                                    // of a tile; a CTA holds half of each operand
 constexpr int PAIR_WARPS = 8;                                     // of the epilogue
-constexpr int TURN_BYTES = 2048, BIAS_BYTES = 512;                // per epilogue warp: 32 rows x 64 bytes, 128 bias values
-constexpr int PAIR_OFF_TURN = PAIR_STAGES * PAIR_STAGE, PAIR_OFF_BIAS = PAIR_OFF_TURN + PAIR_WARPS * TURN_BYTES,
-              PAIR_OFF_BARS = PAIR_OFF_BIAS + PAIR_WARPS * BIAS_BYTES, PAIR_SMEM = 1024 + PAIR_OFF_BARS + BAR_BYTES;
-static_assert(PAIR_SMEM <= 227 * 1024, "shared memory");
+constexpr int TURN_BYTES = 2048, BIAS_BYTES = 512;                // per epilogue warp: 32 rows x 64 bytes, bias of its columns
+// What a tile of BN columns takes: bytes of a stage that a CTA loads, stages, places in shared memory.
+template <int BN> struct PairTile {
+  static constexpr int R_BYTES = 128 * BK * 2, STAGE = R_BYTES + BN / 2 * BK * 2, STAGES = BN == 256 ? 6 : 8;
+  static constexpr int OFF_TURN = STAGES * STAGE, OFF_BIAS = OFF_TURN + PAIR_WARPS * TURN_BYTES, OFF_BARS = OFF_BIAS + PAIR_WARPS * BIAS_BYTES;
+  static constexpr int SMEM = 1024 + OFF_BARS + BAR_BYTES;
+  static_assert(SMEM <= 227 * 1024 && STAGE % 1024 == 0, "shared memory");
+};
 
 struct PairArgs {
   int n_steps, n_rt, n_ct, n_tiles, r_mn, c_mn;
@@ -550,34 +559,35 @@ __device__ __forceinline__ void load_rows(uint8_t *turn, uint32_t (&w)[16], cons
 }
 
 // ACT: the activation of a layer; -1: the product alone.
-template <typename T, int ACT>
+template <typename T, int ACT, int BN>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Out o,
                 const __grid_constant__ PairArgs g) {
+  using P = PairTile<BN>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t *base_ptr = smem_raw + (base - raw);
-  const uint32_t bars = base + PAIR_OFF_BARS;      // full[6] empty[6] acc_full[2] acc_empty[2]
+  const uint32_t bars = base + P::OFF_BARS;      // full[8] empty[8] acc_full[2] acc_empty[2]
   auto full = [&](int i) { return bars + 8u * i; };
   auto empty = [&](int i) { return bars + 64u + 8u * i; };
   auto acc_full = [&](int i) { return bars + 128u + 8u * i; };
   auto acc_empty = [&](int i) { return bars + 144u + 8u * i; };
   const uint32_t tmem_slot = bars + 196u;
-  volatile unsigned *abort_word = reinterpret_cast<volatile unsigned *>(base_ptr + PAIR_OFF_BARS + 192);
+  volatile unsigned *abort_word = reinterpret_cast<volatile unsigned *>(base_ptr + P::OFF_BARS + 192);
   unsigned *err = &g_linear_error;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
 
   if (warp == 1 && lane == 0) { prefetch_map(&map_r); prefetch_map(&map_c); }
   if (warp == 0) {
-    if (lane < PAIR_STAGES) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
-    else if (lane < 8) { mbar_init(acc_full(lane - 6), 1); mbar_init(acc_empty(lane - 6), 2 * PAIR_WARPS); }
-    else if (lane == 8) *abort_word = 0u;
+    if (lane < 8) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
+    else if (lane < 10) { mbar_init(acc_full(lane - 8), 1); mbar_init(acc_empty(lane - 8), 2 * PAIR_WARPS); }
+    else if (lane == 10) *abort_word = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;                   // issues the MMAs of the pair
-  if (warp == 2) tmem_alloc<true>(tmem_slot, 512);
+  if (warp == 2) tmem_alloc<true>(tmem_slot, 2 * BN);
   tc_fence_before();
   __syncthreads();
   cluster_sync_all();                              // the barriers of both CTAs exist before either arrives at the other's
@@ -596,16 +606,16 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     for (int t = tile0; t < g.n_tiles && alive; t += tile_step) {
       int rt, ct;
       tile_at(g, t, rt, ct);
-      const int row = rt * PAIR_TILE + (int)rank * 128, col = ct * PAIR_TILE + (int)rank * 128;
+      const int row = rt * PAIR_ROWS + (int)rank * 128, col = ct * BN + (int)rank * (BN / 2);
       for (int k = 0; k < g.n_steps; ++k) {
         if (!mbar_wait_warp(empty(s), ph, abort_word, err, ERR_EMPTY)) { alive = false; break; }
         if (lane == 0) {
-          if (leader) mbar_expect_tx(full(s), 2u * PAIR_STAGE);
-          const uint32_t dst = base + (uint32_t)(s * PAIR_STAGE);
+          if (leader) mbar_expect_tx(full(s), 2u * P::STAGE);
+          const uint32_t dst = base + (uint32_t)(s * P::STAGE);
           load_operand<true>(dst, &map_r, full(s), g.r_mn, row, 128, k * BK);
-          load_operand<true>(dst + PAIR_STAGE / 2, &map_c, full(s), g.c_mn, col, 128, k * BK);
+          load_operand<true>(dst + P::R_BYTES, &map_c, full(s), g.c_mn, col, BN / 2, k * BK);
         }
-        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        if (++s == P::STAGES) { s = 0; ph ^= 1u; }
       }
     }
     if (*abort_word != 0u) {   // loads in flight must land before the shared memory goes away
@@ -621,37 +631,37 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       const int buf = n & 1;
       if (!mbar_wait_warp(acc_empty(buf), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_word, err, ERR_ACC_EMPTY)) break;
       tc_fence_after();
-      const uint32_t d = tmem + (uint32_t)(buf * PAIR_TILE);
+      const uint32_t d = tmem + (uint32_t)(buf * BN);
       for (int k = 0; k < g.n_steps; ++k) {
         if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
         tc_fence_after();
-        const uint32_t st = base + (uint32_t)(s * PAIR_STAGE);
-        const uint32_t a = operand_lo(st, g.r_mn), b = operand_lo(st + PAIR_STAGE / 2, g.c_mn);
+        const uint32_t st = base + (uint32_t)(s * P::STAGE);
+        const uint32_t a = operand_lo(st, g.r_mn), b = operand_lo(st + P::R_BYTES, g.c_mn);
         if (elect_one()) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) umma<true, false>(d, a + (uint32_t)j * a_step, hi, b + (uint32_t)j * b_step, hi, g.idesc, (k > 0 || j > 0) ? 1u : 0u);
           umma_commit<true>(empty(s), 3);
         }
         __syncwarp();
-        if (++s == PAIR_STAGES) { s = 0; ph ^= 1u; }
+        if (++s == P::STAGES) { s = 0; ph ^= 1u; }
       }
       if (alive && elect_one()) umma_commit<true>(acc_full(buf), 3);
       __syncwarp();
     }
   } else if (warp >= 4) {
     const int ew = warp - 4, q = warp & 3, half = ew >> 2;
-    uint8_t *turn = base_ptr + PAIR_OFF_TURN + ew * TURN_BYTES;
-    float *bias = reinterpret_cast<float *>(base_ptr + PAIR_OFF_BIAS + ew * BIAS_BYTES);
+    uint8_t *turn = base_ptr + P::OFF_TURN + ew * TURN_BYTES;
+    float *bias = reinterpret_cast<float *>(base_ptr + P::OFF_BIAS + ew * BIAS_BYTES);
     const int n_blk = (o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK;
     int n = 0;
     for (int t = tile0; t < g.n_tiles; t += tile_step, ++n) {
       int rt, ct;
       tile_at(g, t, rt, ct);
       const int buf = n & 1;
-      const int row0 = rt * PAIR_TILE + (int)rank * 128 + q * 32, col0 = ct * PAIR_TILE + half * 128, rows = o.rows - row0;
+      const int row0 = rt * PAIR_ROWS + (int)rank * 128 + q * 32, col0 = ct * BN + half * (BN / 2), rows = o.rows - row0;
       if (ACT >= 0) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < BN / 64; ++j) {
           const int c = col0 + j * 32 + lane;
           bias[j * 32 + lane] = !o.bias || c >= o.cols ? 0.f : o.bias_f32 ? reinterpret_cast<const float *>(o.bias)[c] : Elem<T>::load((const T *)o.bias + c);
         }
@@ -660,11 +670,11 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
       if (!mbar_wait_warp(acc_full(buf), (uint32_t)(n >> 1) & 1u, abort_word, err, ERR_ACC_FULL)) break;
       tc_fence_after();
 #pragma unroll 1
-      for (int ch = 0; ch < 4; ++ch) {
+      for (int ch = 0; ch < BN / 64; ++ch) {
         const int c = col0 + ch * 32, cols = o.cols - c;
         if (cols <= 0 || rows <= 0) break;
         uint32_t v[32];
-        tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * PAIR_TILE + half * 128 + ch * 32), v);
+        tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * (BN / 2) + ch * 32), v);
         uint32_t res[16];
         if (ACT >= 0 && o.residual) {      // on its way while the accumulator is read
           const uint8_t *src = (const uint8_t *)o.residual + ((long long)row0 * o.residual_stride + c) * 2;
@@ -759,7 +769,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
   cluster_sync_all();
   if (warp == 2) {
     tc_fence_after();
-    tmem_free<true>(tmem, 512);
+    tmem_free<true>(tmem, 2 * BN);
   }
 }
 
@@ -850,24 +860,24 @@ template <typename T> cudaError_t launch_rows(const LinearProblem &p, cudaStream
   return cudaLaunchKernelEx(&cfg, kern, (const T *)p.r.ptr, p.r.stride, (const T *)p.c.ptr, p.c.stride, p.red, out_of(p, 1));
 }
 
-template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+template <typename T, int ACT, int BN> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
   CUtensorMap mr, mc;
-  if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, 128) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, 128)) {
+  if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, 128) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, BN / 2)) {
     *detail = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = pair_kernel<T, ACT>;
+  auto kern = pair_kernel<T, ACT, BN>;
   cudaError_t e = allow_smem((const void *)kern);
   if (e != cudaSuccess) return e;
   PairArgs g;
   g.n_steps = (p.red + BK - 1) / BK;
-  g.n_rt = (p.rows + PAIR_TILE - 1) / PAIR_TILE; g.n_ct = (p.cols + PAIR_TILE - 1) / PAIR_TILE;
+  g.n_rt = (p.rows + PAIR_ROWS - 1) / PAIR_ROWS; g.n_ct = (p.cols + BN - 1) / BN;
   g.n_tiles = g.n_rt * g.n_ct;
   g.r_mn = p.r.mn; g.c_mn = p.c.mn;
-  g.idesc = instruction(p.dtype, p.r.mn, p.c.mn, 256, 256);
+  g.idesc = instruction(p.dtype, p.r.mn, p.c.mn, PAIR_ROWS, BN);
   cudaLaunchConfig_t cfg = {};
   cfg.blockDim = dim3(PAIR_THREADS);
-  cfg.dynamicSmemBytes = PAIR_SMEM; cfg.stream = s;
+  cfg.dynamicSmemBytes = PairTile<BN>::SMEM; cfg.stream = s;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -877,14 +887,17 @@ template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, E
   cfg.gridDim = dim3(2u * (unsigned)std::min(g.n_tiles, SMS / 2));
   return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 8), g);
 }
-template <typename T> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
-  if (!p.layer) return launch_pair<T, -1>(p, enc, s, detail);
+template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  return bn == 256 ? launch_pair<T, ACT, 256>(p, enc, s, detail) : bn == 128 ? launch_pair<T, ACT, 128>(p, enc, s, detail) : launch_pair<T, ACT, 64>(p, enc, s, detail);
+}
+template <typename T> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  if (!p.layer) return launch_pair<T, -1>(p, bn, enc, s, detail);
   switch (p.act) {
-    case WINOCONV_ACT_RELU: return launch_pair<T, WINOCONV_ACT_RELU>(p, enc, s, detail);
-    case WINOCONV_ACT_GELU: return launch_pair<T, WINOCONV_ACT_GELU>(p, enc, s, detail);
-    case WINOCONV_ACT_GELU_TANH: return launch_pair<T, WINOCONV_ACT_GELU_TANH>(p, enc, s, detail);
-    case WINOCONV_ACT_SILU: return launch_pair<T, WINOCONV_ACT_SILU>(p, enc, s, detail);
-    default: return launch_pair<T, WINOCONV_ACT_NONE>(p, enc, s, detail);
+    case WINOCONV_ACT_RELU: return launch_pair<T, WINOCONV_ACT_RELU>(p, bn, enc, s, detail);
+    case WINOCONV_ACT_GELU: return launch_pair<T, WINOCONV_ACT_GELU>(p, bn, enc, s, detail);
+    case WINOCONV_ACT_GELU_TANH: return launch_pair<T, WINOCONV_ACT_GELU_TANH>(p, bn, enc, s, detail);
+    case WINOCONV_ACT_SILU: return launch_pair<T, WINOCONV_ACT_SILU>(p, bn, enc, s, detail);
+    default: return launch_pair<T, WINOCONV_ACT_NONE>(p, bn, enc, s, detail);
   }
 }
 
@@ -894,19 +907,28 @@ using namespace linear;
 
 bool linear_by_rows(long long rows, int layer, bool z8) { return layer && rows <= MOST_ROWS && !z8; }
 
-// The form with the smallest estimated time (us).  The constants are a fit to every form's time on 180 problems (B200, bf16: 3 to
-// 2048 rows, 500 to 16384 columns, reductions of 64 to 25088, the three placements of the operands; launches in a row, operands from
-// HBM): the form chosen takes 1.016 times the fastest one's time on geometric average and 1.15 times at worst.
+// The form with the smallest estimated time (us).  The constants are a fit to every form's time on 204 problems (B200, bf16: 3 to
+// 8192 rows, 500 to 16384 columns, reductions of 64 to 25088, the three placements of the operands; launches in a row, operands from
+// HBM): the form chosen takes 1.026 times the fastest one's time on geometric average and 1.25 times at worst.
 LinearPlan linear_plan(const LinearProblem &p) {
   LinearPlan plan = {};
   plan.by_rows = linear_by_rows(p.rows, p.layer, p.z8 != nullptr);
   if (plan.by_rows) return plan;
   auto over = [](long long a, long long b) { return (a + b - 1) / b; };
-  const long long n_ct = over(p.cols, BC), n_steps = over(p.red, BK);
+  const long long n_steps = over(p.red, BK);
   const double memory = 2.0 + 2.0 * ((double)p.rows * p.red + (double)p.cols * p.red + (double)p.rows * p.cols) / 6.2e6;
-  const double pair_waves = (double)over(over(p.rows, PAIR_TILE) * over(p.cols, PAIR_TILE), SMS / 2);
-  plan.pair = 1;
-  double best = std::max(memory, 4.11 + pair_waves * (0.36 * n_steps + 0.33));
+  double best = 0;
+  // pairs: a step's time is the tensor pipe's for 256 columns, below that the L2's (24 and 20 KB a CTA at 14.5 TB/s in all)
+  const struct { int bn; double step; } pairs[3] = {{256, 0.33}, {128, 0.20}, {64, 0.18}};
+  for (const auto &q : pairs) {
+    if (q.bn == 64 && p.c.mn) continue;      // an MN-major operand comes in 64s: a CTA's half would be 32
+    const double t = std::max(memory, 3.5 + (double)over(over(p.rows, PAIR_ROWS) * over(p.cols, q.bn), SMS / 2) * (n_steps * q.step + 0.3));
+    if (plan.pair == 0 || t < best) {
+      best = t;
+      plan.pair = q.bn;
+    }
+  }
+  const long long n_ct = over(p.cols, BC);
   for (int rows = p.r.mn ? 64 : 16; rows <= 256; rows *= 2) {
     const long long n_rt = over(p.rows, rows);
     if (rows < 256 && n_rt > 16) continue;                                   // many small tiles: never the fastest
@@ -916,8 +938,8 @@ LinearPlan linear_plan(const LinearProblem &p) {
         const int slots = per_sm * (split < 4 ? SMS : split == 4 ? (per_sm == 1 ? 132 : 142) : (per_sm == 1 ? 120 : 132));
         const double ctas = (double)(n_rt * n_ct * split), full = ctas / slots, waves = full <= 3 ? std::ceil(full) : full + 0.5;
         const double stage = C_BYTES + rows * BK * 2, shared = std::max(1.0, std::min(ctas, (double)slots) / SMS);
-        const double step = std::max(0.363, stage * shared * 9.5e-6);        // what a step waits for, or an SM's share of L2
-        const double end = 0.035 * rows + (split > 1 ? 1.2 : 0.0) + 0.28 * split;
+        const double step = std::max(0.36, stage * shared * 9.8e-6);         // what a step waits for, or an SM's share of L2
+        const double end = 0.036 * rows + (split > 1 ? 1.2 : 0.0) + 0.24 * split;
         const double t = std::max(memory, waves * ((double)over(n_steps, split) * step + end));
         if (t < best) {
           best = t;
@@ -937,7 +959,7 @@ cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaSt
   if (plan.by_rows) return p.dtype == WINOCONV_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
-  if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, enc, s, detail) : launch_pair<__nv_bfloat16>(p, enc, s, detail);
+  if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, plan.pair, enc, s, detail) : launch_pair<__nv_bfloat16>(p, plan.pair, enc, s, detail);
   return p.dtype == WINOCONV_F16 ? launch_cluster<__half>(p, plan, enc, s, detail) : launch_cluster<__nv_bfloat16>(p, plan, enc, s, detail);
 }
 

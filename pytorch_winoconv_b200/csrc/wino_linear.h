@@ -26,9 +26,8 @@ struct LinearProblem {
   uint8_t *z8, *z8_scale;    // pre-activation in 8 bits [rows][cols] and its scales [rows][ceil(cols / 32)], or null
   long long residual_stride, y_stride, z_stride;
 };
-// pair: a tile of 256 x 256 by two CTAs, tiles walked by a persistent grid.  Else a tile of `tile_rows` x 128 by a cluster of
-// `split` CTAs that share its reduction.
-// by_rows: a layer's few rows without the tensor cores.
+// pair: columns (256, 128 or 64) of a tile of 256 rows by two CTAs, tiles walked by a persistent grid.  Else a tile of `tile_rows` x
+// 128 by a cluster of `split` CTAs that share its reduction.  by_rows: a layer's few rows without the tensor cores.
 struct LinearPlan {
   int by_rows, pair;
   int tile_rows, split, stages;

@@ -62,7 +62,8 @@ def check(got, want, act, dtype, extra=None):
 
 SHAPES = [(1, 64, 128), (1, 1, 1), (1, 1000, 1531), (1, 4103, 130), (2, 33, 7), (2, 4608, 1001), (3, 4096, 250), (16, 72, 136), (17, 129, 131), (31, 520, 2048), (64, 2048, 129),
           (127, 40, 64), (128, 64, 128), (129, 65, 129), (130, 777, 1000), (257, 200, 520), (1000, 136, 96), (1025, 100, 300), (513, 1024, 768),
-          (1301, 72, 1531), (2000, 129, 1100), (1281, 1801, 1537), (1536, 1600, 1792)]
+          (1301, 72, 1531), (2000, 129, 1100), (1281, 1801, 1537), (1536, 1600, 1792),
+          (300, 2056, 4001), (510, 712, 8000), (4100, 520, 264)]
 
 
 @gpu
