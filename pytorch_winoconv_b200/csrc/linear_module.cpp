@@ -179,8 +179,10 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear: the gradients are not differentiable again (create_graph=True)");
     at::AutoDispatchBelowADInplaceOrView no_graph;
-    const auto saved = ctx->get_saved_variables();
+    auto saved = ctx->get_saved_variables();
     const auto layer = ctx->saved_data["layer"].toIntVector();
+    for (int i = layer[PACK] ? 0 : 1; i < 4; ++i)      // dense, unless a hook on saved tensors has laid them out anew
+      if (saved[i].defined()) saved[i] = saved[i].contiguous();
     const auto type = (at::ScalarType)layer[X_TYPE], w_type = (at::ScalarType)layer[W_TYPE];
     const int act = (int)layer[ACT];
     const bool pack = layer[PACK] != 0, slope = act != WINOCONV_ACT_NONE;

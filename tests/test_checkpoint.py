@@ -85,6 +85,21 @@ def test_views(dtype):
 
 
 @gpu
+def test_more_values_than_32_bits_count():
+    for cols in (4104, 4099):      # by vectors and one by one
+        rows = 2 ** 31 // cols + 100
+        x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+        x[-50:] = torch.randn(50, cols, device="cuda").bfloat16()
+        q, scale = checkpoint.pack(x)
+        part = checkpoint.pack(x[-50:].clone())
+        assert torch.equal(q[-50:].view(torch.uint8), part[0].view(torch.uint8)) and torch.equal(scale[-50:].view(torch.uint8), part[1].view(torch.uint8))
+        del x
+        got = checkpoint.unpack(q, scale)
+        assert torch.equal(got[-50:], checkpoint.unpack(*part)) and got[:50].abs().max() == 0
+        del got, q, scale
+
+
+@gpu
 def test_empty_streams_and_graphs():
     q, scale = checkpoint.pack(torch.empty(0, 40, dtype=torch.float16, device="cuda"))
     assert q.shape == (0, 40) and scale.shape == (0, 2) and checkpoint.unpack(q, scale).shape == (0, 40)

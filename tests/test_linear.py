@@ -397,6 +397,102 @@ def test_streams_and_graphs():
 
 
 @gpu
+def test_more_values_than_32_bits_count():
+    """2^31 outputs and more: the last rows are those of a call on them alone, forward and backward."""
+    rows, k, n, dtype = 262_147, 64, 8_200, torch.bfloat16
+    assert rows * n > 2 ** 31
+    x, w, b, _ = make(rows, k, n, dtype, residual=False)
+    part = x[-300:].clone()
+    x.requires_grad_()
+    y = lin.linear(x, w, b, activation="relu", checkpoint="e4m3")
+    want, = (lin.linear(part.requires_grad_(), w, b, activation="relu", checkpoint="e4m3"),)
+    assert torch.equal(y[-300:], want)
+    gy = torch.zeros_like(y)
+    gy[-300:] = ints((300, n), 9, 4, 2.0 ** -6, dtype)
+    dx, = torch.autograd.grad(y, x, gy)
+    dp, = torch.autograd.grad(want, part, gy[-300:].clone())
+    assert torch.equal(dx[-300:], dp) and dx[:-300].abs().max() == 0
+    assert capi.read_device_error() == 0
+
+
+@gpu
+def test_a_first_call_that_is_captured():
+    """A fresh process whose first calls of the layer are in a capture, forward and backward: kernels are loaded and attributes set
+    without a word to the stream, and the replay gives the eager values."""
+    code = """
+import torch
+from pytorch_winoconv_b200 import capi, linear
+torch.manual_seed(0)
+x = torch.randn(40, 72, device="cuda").half()
+w = torch.randn(104, 72, device="cuda").half().requires_grad_()
+gy = torch.randn(40, 104, device="cuda").half()
+def step():
+    leaf = x.detach().requires_grad_()
+    y = linear.linear(leaf, w, activation="gelu", checkpoint="e4m3")
+    return [y.detach(), *torch.autograd.grad(y, (leaf, w), gy)]
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g2 = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g2):
+    out2 = step()
+g.replay(); g2.replay(); torch.cuda.synchronize()
+want = step()
+assert all(torch.equal(a, b) for a, b in zip(out, want)) and all(torch.equal(a, b) for a, b in zip(out2, want))
+assert capi.read_device_error() == 0
+print("captured")
+"""
+    import os
+    import subprocess
+    import sys
+    done = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
+@gpu
+def test_threads_inference_mode_and_hooks_on_saved_tensors():
+    import threading
+    x, w, b, r = make(130, 136, 264, torch.float16)
+    gy = ints((130, 264), 9, 4, 2.0 ** -6, torch.float16)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+        y = lin.linear(*leaves, activation="silu", checkpoint="e4m3")
+        return [y.detach(), *torch.autograd.grad(y, leaves, gy)]
+
+    want, got = step(), {}
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = [step() for _ in range(20)][-1]
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 3 and all(torch.equal(a, c) for v in got.values() for a, c in zip(v, want))
+    with torch.inference_mode():
+        y = lin.linear(x.clone(), w, b, r, activation="silu")
+    assert torch.equal(y, want[0])
+    with torch.autograd.graph.save_on_cpu():      # what is kept goes to the host and comes back
+        assert all(torch.equal(a, c) for a, c in zip(step(), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.stack([t.view(torch.uint8)] * 2, -1)[..., 0].view(t.dtype)
+                                                  if t.element_size() == 1 else t):      # laid out with gaps
+        assert all(torch.equal(a, c) for a, c in zip(step(), want))
+    # one tensor in several places: as the input and the residual, and as the input and the weight
+    s = ints((64, 64), 3, 4, 0.25, torch.float16).requires_grad_()
+    g = ints((64, 64), 4, 4, 2.0 ** -6, torch.float16)
+    ds, = torch.autograd.grad(lin.linear(s, s, None, s), s, g)
+    gd, sd = g.double(), s.detach().double()
+    parts = [gd @ sd, gd.t() @ sd, gd]
+    assert ((ds.double() - sum(parts)).abs() <= 3 * sum(half_step(p, torch.float16) for p in parts) + half_step(sum(parts), torch.float16)).all()
+
+
+@gpu
 def test_gradients_accumulate_and_chain():
     """A feed-forward block as it would be used: two layers, the skip connection in the second's epilogue, shared weights."""
     dtype = torch.float16
