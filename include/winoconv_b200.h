@@ -319,6 +319,13 @@ WINOCONV_API int winoconv_e4m3_pack(int dtype, const void *x, int64_t x_stride, 
 WINOCONV_API int winoconv_e4m3_unpack(int dtype, const void *q, const void *scale, int64_t rows, int32_t cols, void *x, int64_t x_stride, void *stream);
 
 /*
+ * What a ReLU's gradient needs of its result, a bit for each value: bits[i / 8] has bit i % 8 set where y[i] > 0; and gx[i] = gy[i] times
+ * that bit.  n values of dtype F16 or BF16 without gaps, y, gy and gx on 16 bytes, (n + 7) / 8 bytes of bits (behind the last value: 0).
+ */
+WINOCONV_API int winoconv_sign_pack(int dtype, const void *y, int64_t n, void *bits, void *stream);
+WINOCONV_API int winoconv_sign_apply(int dtype, const void *gy, const void *bits, int64_t n, void *gx, void *stream);
+
+/*
  * The per-position batched GEMM on its own: m[p][t][k] = sum_c v[p][t][c] * u[p][k][c],
  * fp32 accumulate.  v [positions][tiles][c_pad], u [positions][k_out][c_pad] in `dtype`,
  * m [positions][tiles][k_out] in `product_dtype`.  c_pad must be a multiple of 8.

@@ -33,6 +33,7 @@ EXPORTED_SYMBOLS = (
     "winoconv_backward_data", "winoconv_backward_weight", "winoconv_to_channels_last", "winoconv_to_channels_first",
     "winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation", "winoconv_linear_backward_data",
     "winoconv_linear_backward_weight", "winoconv_pad_rows", "winoconv_e4m3_pack", "winoconv_e4m3_unpack",
+    "winoconv_sign_pack", "winoconv_sign_apply",
 )
 
 
@@ -114,7 +115,9 @@ def lib() -> ctypes.CDLL:
     L.winoconv_pad_rows.argtypes = [POINTER(Rows), c_int32, c_void_p]
     L.winoconv_e4m3_pack.argtypes = [c_int, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p]
     L.winoconv_e4m3_unpack.argtypes = [c_int, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]
-    for name in ("winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation",
+    L.winoconv_sign_pack.argtypes = [c_int, c_void_p, c_int64, c_void_p, c_void_p]
+    L.winoconv_sign_apply.argtypes = [c_int, c_void_p, c_void_p, c_int64, c_void_p, c_void_p]
+    for name in ("winoconv_sign_pack", "winoconv_sign_apply", "winoconv_linear_forward", "winoconv_linear_backward_ws", "winoconv_linear_backward_activation",
                  "winoconv_linear_backward_data", "winoconv_linear_backward_weight", "winoconv_pad_rows", "winoconv_e4m3_pack",
                  "winoconv_e4m3_unpack"):
         getattr(L, name).restype = c_int

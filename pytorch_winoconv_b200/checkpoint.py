@@ -6,8 +6,8 @@ most 2^-4 for all but the values that are 2^-13 or less of their block's largest
 bits, so what comes back is held by float16 and bfloat16 without another rounding.  Infinities and NaN come back as NaN; a value that
 rounds up beyond the type's largest (65504 in float16) comes back as that largest.
 
-``linear.Linear(checkpoint="e4m3")`` uses it; :func:`pack` and :func:`unpack` are the operators themselves, for a program's own
-autograd functions.
+``linear.Linear``, ``conv.Conv2d`` and ``conv.Conv3d`` use it with ``checkpoint="e4m3"`` (a convolution packs the channels of each
+pixel: fewer than 32 save less); :func:`pack` and :func:`unpack` are the operators themselves, for a program's own autograd functions.
 """
 from __future__ import annotations
 

@@ -26,8 +26,8 @@ Backward (the reference left only traces of one: ``include/splitstrideone/split_
   stride grid), the weight gradient by one tensor-core GEMM per filter tap (``winoconv_gemm_batched``), the bias gradient a sum.
 
 A fused ReLU is differentiated through the stored output; the fused max-pool is forward only.  With ``checkpoint="e4m3"`` a 16-bit
-layer keeps its input in eight bits (and the ReLU as a byte for each value) instead of the tensors themselves: half the memory, the
-result and the data gradient unchanged, the weight gradient that of an input rounded to four significant bits.
+layer keeps its input in eight bits (and the ReLU as a bit for each value) instead of the tensors themselves: little more than half
+the memory, the result and the data gradient unchanged, the weight gradient that of an input rounded to four significant bits.
 ``groups != 1`` and dilation raise (the reference accepts ``groups`` and silently computes groups = 1).
 """
 from __future__ import annotations

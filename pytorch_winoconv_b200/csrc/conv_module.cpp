@@ -108,11 +108,15 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
                             const at::Tensor &x_cl, const std::shared_ptr<ConvRunner::Entry> &entry, const at::Tensor &weight,
                             const std::optional<at::Tensor> &bias, bool relu, bool pack) {
     at::Tensor y = runner->run(*entry, x_cl, weight, bias, weight.requires_grad());
-    if (pack) {      // x in eight bits where the weight gradient reads it, the ReLU as a byte for each value
+    if (pack) {      // x in eight bits where the weight gradient reads it, the ReLU as a bit for each value
       at::AutoDispatchBelowADInplaceOrView no_graph;
-      at::Tensor q, scale;
+      at::Tensor q, scale, bits;
       if (weight.requires_grad()) std::tie(q, scale) = e4m3_pack(x_cl.movedim(1, -1));
-      ctx->save_for_backward({q, scale, relu ? y > 0 : at::Tensor()});
+      if (relu) {      // in the order of memory: y is channels last without gaps
+        bits = empty_bytes((uint64_t)(y.numel() + 7) / 8, y);
+        check_abi(winoconv_sign_pack(code_of(y.scalar_type()), y.data_ptr(), y.numel(), bits.data_ptr(), stream_of()), "winoconv_sign_pack");
+      }
+      ctx->save_for_backward({q, scale, bits});
       ctx->saved_data["x_sizes"] = x.sizes().vec();
       ctx->saved_data["x_type"] = (int64_t)x.scalar_type();
     } else ctx->save_for_backward({x, relu ? y : at::Tensor()});
@@ -140,7 +144,14 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
       // (without the weight gradient nothing reads x: a tensor of its sizes stands for it)
       const at::Tensor x = saved[0].defined() ? e4m3_unpack(saved[0], saved[1], runner->type_for(x_type)).movedim(-1, 1)
                                               : at::empty({1}, grads[0].options().dtype(x_type)).expand(ctx->saved_data["x_sizes"].toIntVector());
-      g = runner->backward(saved[2].defined() ? grads[0] * saved[2].to(grads[0].scalar_type()) : grads[0], x, at::Tensor(), weight, bias, nx, nw && saved[0].defined(), nb);
+      at::Tensor gy = grads[0];
+      if (saved[2].defined()) {
+        const at::ScalarType type = runner->type_for(x_type);
+        const at::Tensor dense = aligned(dense_channels_last(gy, type, stream_of()));
+        gy = at::empty_like(dense);
+        check_abi(winoconv_sign_apply(code_of(type), dense.data_ptr(), saved[2].contiguous().data_ptr(), gy.numel(), gy.data_ptr(), stream_of()), "winoconv_sign_apply");
+      }
+      g = runner->backward(gy, x, at::Tensor(), weight, bias, nx, nw && saved[0].defined(), nb);
       if (g[0].defined() && g[0].scalar_type() != x_type) g[0] = g[0].to(x_type);
     } else g = runner->backward(grads[0], saved[0], saved[1], weight, bias, nx, nw, nb);
     out[1] = g[0];

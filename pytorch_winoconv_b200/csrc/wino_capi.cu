@@ -1050,6 +1050,29 @@ int winoconv_e4m3_unpack(int dtype, const void *q, const void *scale, int64_t ro
   return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "e4m3 unpack launch");
 }
 
+static int check_signs(int dtype, const void *a, const void *b, const void *bits, int64_t n) {
+  if (!a || !b || !bits) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null tensor");
+  if (!is16(dtype)) return fail(WINOCONV_ERR_UNSUPPORTED, "signs are kept of f16 or bf16 values");
+  if (n <= 0) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "sizes must be positive");
+  if (n > (1LL << 40)) return fail(WINOCONV_ERR_UNSUPPORTED, "tensor too large");
+  if (!aligned16(a) || !aligned16(b)) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "tensors must be 16-byte aligned");
+  return winoconv_device_check();
+}
+
+int winoconv_sign_pack(int dtype, const void *y, int64_t n, void *bits, void *stream) {
+  const int st = check_signs(dtype, y, y, bits, n);
+  if (st != WINOCONV_OK) return st;
+  const cudaError_t e = launch_sign_pack(dtype, y, n, (uint8_t *)bits, (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "sign pack launch");
+}
+
+int winoconv_sign_apply(int dtype, const void *gy, const void *bits, int64_t n, void *gx, void *stream) {
+  const int st = check_signs(dtype, gy, gx, bits, n);
+  if (st != WINOCONV_OK) return st;
+  const cudaError_t e = launch_sign_apply(dtype, gy, (const uint8_t *)bits, n, gx, (cudaStream_t)stream);
+  return e == cudaSuccess ? WINOCONV_OK : cuda_fail(e, "sign apply launch");
+}
+
 int winoconv_gemm_batched(int dtype, int product_dtype, int gemm_engine, int positions, int64_t tiles, int c_pad,
                           int k_out, const void *v, const void *u, void *m, void *stream) {
   if (!v || !u || !m) return fail(WINOCONV_ERR_INVALID_ARGUMENT, "null operand");

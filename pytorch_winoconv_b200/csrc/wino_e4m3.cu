@@ -192,6 +192,54 @@ __global__ void __launch_bounds__(THREADS) unpack_ragged_kernel(const uint8_t *q
   }
 }
 
+// ---- a ReLU's signs ---------------------------------------------------------------------------------------------------
+// Eight values and their byte a thread, four times.
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sign_pack_kernel(const T *y, unsigned long long n, uint8_t *bits) {
+  grid_start();
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const unsigned long long i = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x + u * THREADS;
+    if (i * 8 >= n) return;
+    uint32_t w[4] = {0u, 0u, 0u, 0u};
+    if (i * 8 + 8 <= n) {
+      const uint4 v = reinterpret_cast<const uint4 *>(y)[i];
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else {
+      for (int j = 0; j < (int)(n - i * 8); ++j) w[j >> 1] |= (uint32_t)reinterpret_cast<const uint16_t *>(y)[i * 8 + j] << (16 * (j & 1));
+    }
+    uint32_t b = 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = Pair16<T>::unpack(w[j]);
+      b |= (f.x > 0.f ? 1u : 0u) << (2 * j) | (f.y > 0.f ? 2u : 0u) << (2 * j);
+    }
+    bits[i] = (uint8_t)b;
+  }
+}
+template <typename T>
+__global__ void __launch_bounds__(THREADS) sign_apply_kernel(const T *gy, const uint8_t *bits, unsigned long long n, T *gx) {
+  grid_start();
+#pragma unroll
+  for (int u = 0; u < UNROLL; ++u) {
+    const unsigned long long i = (unsigned long long)blockIdx.x * (THREADS * UNROLL) + threadIdx.x + u * THREADS;
+    if (i * 8 >= n) return;
+    const uint32_t b = bits[i];
+    if (i * 8 + 8 <= n) {
+      const uint4 v = reinterpret_cast<const uint4 *>(gy)[i];
+      uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {      // a product, not a choice: what is not finite stays visible
+        const float2 f = Pair16<T>::unpack(w[j]);
+        w[j] = Pair16<T>::round(f.x * (float)((b >> (2 * j)) & 1u), f.y * (float)((b >> (2 * j + 1)) & 1u));
+      }
+      reinterpret_cast<uint4 *>(gx)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      for (int j = 0; j < (int)(n - i * 8); ++j) Elem<T>::store(gx + i * 8 + j, Elem<T>::load(gy + i * 8 + j) * (float)((b >> j) & 1u));
+    }
+  }
+}
+
 // Rows copied with zeros behind them, eight values a thread; the second matrix by blocks of its own.
 __global__ void __launch_bounds__(THREADS) pad_rows_kernel(const __grid_constant__ PadRows p) {
   const auto &m = p.m[blockIdx.y];
@@ -422,6 +470,16 @@ cudaError_t launch_pad_rows(const PadRows &p, cudaStream_t s) {
   unsigned long long n = 1;
   for (int i = 0; i < p.count; ++i) n = std::max(n, (unsigned long long)p.m[i].rows * (unsigned long long)(p.m[i].y_stride / 8));
   return launch(pad_rows_kernel, dim3((unsigned)std::min<unsigned long long>((n + THREADS - 1) / THREADS, 16 * 148), (unsigned)p.count), s, p);
+}
+cudaError_t launch_sign_pack(int dtype, const void *y, long long n, uint8_t *bits, cudaStream_t s) {
+  const unsigned blocks = blocks_of((unsigned long long)(n + 7) / 8, THREADS * UNROLL);
+  return dtype == WINOCONV_F16 ? launch(sign_pack_kernel<__half>, blocks, s, (const __half *)y, (unsigned long long)n, bits)
+                               : launch(sign_pack_kernel<__nv_bfloat16>, blocks, s, (const __nv_bfloat16 *)y, (unsigned long long)n, bits);
+}
+cudaError_t launch_sign_apply(int dtype, const void *gy, const uint8_t *bits, long long n, void *gx, cudaStream_t s) {
+  const unsigned blocks = blocks_of((unsigned long long)(n + 7) / 8, THREADS * UNROLL);
+  return dtype == WINOCONV_F16 ? launch(sign_apply_kernel<__half>, blocks, s, (const __half *)gy, bits, (unsigned long long)n, (__half *)gx)
+                               : launch(sign_apply_kernel<__nv_bfloat16>, blocks, s, (const __nv_bfloat16 *)gy, bits, (unsigned long long)n, (__nv_bfloat16 *)gx);
 }
 // Runs of rows: multiples of the 32 that a block has in flight, short enough for three waves of four blocks on every SM (so that
 // the last wave costs little; the partial sums stay below a tenth of what is read), at most 65535 of them.

@@ -7,13 +7,18 @@
 //     weight gradient  R = dz and C = x, both read down their columns     dW
 //
 // "Down its columns" is an MN-major operand of the MMA: TMA brings [reduction][64 rows] boxes as they lie, nothing is transposed
-// or copied.
+// or copied.  No form needs scratch or atomics, and each gives the same bits every time.  Three forms, chosen by linear_plan:
 //
-// Cluster kernel: a tile of up to 256 rows x 128 columns by a cluster of CTAs that share its reduction.  The 128 columns (output
-// features) are the M side of the MMA and the rows its N side, so one row costs no more than 16 and the weights, which are what
-// has to be read when rows are few, stream through a ring of TMA stages; the parts of a tile are added up over distributed shared
-// memory, in the same order in every CTA: no scratch, no atomics, the same bits every time.  Two CTAs of an SM keep the memory
-// busy while a third party's sums travel.
+//   row kernel      one or two rows: weights read once by plain loads, FMA                        (bound by HBM)
+//   cluster kernel  few rows, few tiles: 128 columns x up to 256 rows by a cluster of CTAs        (HBM, or the launch)
+//   pair kernel     256 rows x 256, 128 or 64 columns by a CTA pair, persistent                   (tensor pipe, or L2)
+//
+// Cluster kernel.  The 128 columns (output features) are the M side of the MMA and the rows its N side, so one row costs no more
+// than 16 and the weights, which are what has to be read when rows are few, stream through a ring of TMA stages.  The CTAs of a
+// cluster share the reduction; the parts are added up over distributed shared memory in the same order by every CTA, vectors of four
+// read from all peers at once (sending single values to the CTA that finishes a row instead took 17.5 us where this took 10.8: 509 x 1000 x
+// 1531).  Two CTAs to an SM where the ring fits twice.  24 x 4096 x 16384 (f16) 23.5 us, 5.7 TB/s of weights; 64 x 4096 x 4096 10.2 us
+// and 16 x 4096 x 4096 8.1 us, of which the launch, the first loads, the exchange and the end take about 5.
 //
 // Roles: warp 0 TMA, warp 1 MMA issue; then all eight warps move the accumulator to shared memory and add up and store their share
 // of the rows.  Every mbarrier wait is bounded and reports through the error word.

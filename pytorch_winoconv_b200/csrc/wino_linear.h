@@ -68,4 +68,8 @@ cudaError_t launch_act_grad(const ActGrad &a, cudaStream_t s);
 cudaError_t launch_e4m3_pack(int dtype, const void *x, long long x_stride, long long rows, int cols, uint8_t *q, uint8_t *scale, cudaStream_t s);
 cudaError_t launch_e4m3_unpack(int dtype, const uint8_t *q, const uint8_t *scale, long long rows, int cols, void *x, long long x_stride, cudaStream_t s);
 
+// Signs of a ReLU's result, eight to a byte, and a gradient times them.
+cudaError_t launch_sign_pack(int dtype, const void *y, long long n, uint8_t *bits, cudaStream_t s);
+cudaError_t launch_sign_apply(int dtype, const void *gy, const uint8_t *bits, long long n, void *gx, cudaStream_t s);
+
 }  // namespace wino

@@ -2,8 +2,9 @@
 
 The layers that stand between and behind convolutions -- 1x1 heads on pooled features, classifiers, feed-forward blocks -- run on
 the tensor cores like them (``csrc/wino_linear.cu``): 16-bit operands, products and sums in fp32, bias, activation and residual
-applied to the fp32 sums, one rounding at the end.  One row is served by the kernel that streams the weights, thousands by one
-that keeps the tensor cores busy; both take any size and any row stride, and give the same bits every time.
+applied to the fp32 sums, one rounding at the end.  One or two rows are served by a kernel that reads the weights once, a few by
+clusters that share the reduction, thousands by one that keeps the tensor cores busy; all take any size and any row stride, and
+give the same bits every time.
 
 * :func:`linear` -- the operator on tensors; :class:`Linear` -- the ``torch.nn.Linear`` subclass, as ``conv.Conv2d`` is one of
   ``torch.nn.Conv2d``.
@@ -13,7 +14,9 @@ that keeps the tensor cores busy; both take any size and any row stride, and giv
   ``checkpoint="e4m3"`` keeps both in eight bits instead (:mod:`.checkpoint`): half the memory, gradients as if x and the
   pre-activation had been rounded to four significant bits; the forward result is the same.
 
-The gradients are not differentiable again.  There is no CPU path and no library product.
+The gradients are not differentiable again.  There is no CPU path and no library product.  Calls keep nothing but what autograd
+saves: they may run on several threads and streams and in captured graphs.  (As with every operator of torch, a backward pass can only
+be captured when no eager graph of the same parameters, built on another stream, is still alive: torch raises there.)
 """
 from __future__ import annotations
 

@@ -178,20 +178,41 @@ def test_convolution_layers(cls, shape, k, ks, stride, pad, bias, activation, dt
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 7, 8, 9, 1000, 8192, 100_003])
+def test_signs(n, dtype):
+    lib, code = capi.lib(), capi.F16 if dtype == torch.float16 else capi.BF16
+    y = torch.randn(n + 8, device="cuda").to(dtype)
+    y[:n:5] = 0
+    y[:n:11] = -0.0
+    y[n // 2] = float("nan")
+    gy = torch.randn(n, device="cuda").to(dtype)
+    bits = torch.full(((n + 7) // 8 + 3,), 0xAA, dtype=torch.uint8, device="cuda")
+    gx = torch.full((n + 8,), 7.0, dtype=dtype, device="cuda")
+    s = torch.cuda.current_stream().cuda_stream
+    capi.check(lib.winoconv_sign_pack(code, y.data_ptr(), n, bits.data_ptr(), s), "sign_pack")
+    capi.check(lib.winoconv_sign_apply(code, gy.data_ptr(), bits.data_ptr(), n, gx.data_ptr(), s), "sign_apply")
+    on = torch.stack([(bits[:(n + 7) // 8].int() >> i) & 1 for i in range(8)], 1).flatten()
+    assert torch.equal(on[:n].bool(), y[:n] > 0) and on[n:].sum() == 0 and (bits[(n + 7) // 8:] == 0xAA).all()
+    assert torch.equal(gx[:n], gy * (y[:n] > 0).to(dtype)) and (gx[n:] == 7).all()
+    assert capi.read_device_error() == 0
+
+
+@gpu
 def test_what_a_convolution_layer_keeps():
     layer = conv.Conv2d(64, 32, 3, padding=1, activation="relu", checkpoint="e4m3").cuda()
     x = torch.randn(4, 64, 20, 20, device="cuda", requires_grad=True)      # float input: kept as the rounded operand's eight bits
     size = []
     with torch.autograd.graph.saved_tensors_hooks(lambda t: size.append(t.numel() * t.element_size()) or t, lambda t: t):
         y = layer(x)
-    assert sorted(size) == sorted([x.numel(), x.numel() // 32, y.numel()])
+    assert sorted(size) == sorted([x.numel(), x.numel() // 32, y.numel() // 8])
     y.float().sum().backward()
     assert x.grad.dtype == torch.float32 and layer.weight.grad is not None
     layer.weight.requires_grad_(False)
     size.clear()
     with torch.autograd.graph.saved_tensors_hooks(lambda t: size.append(t.numel() * t.element_size()) or t, lambda t: t):
         y = layer(x)
-    assert size == [y.numel()]
+    assert size == [y.numel() // 8]
     plain = conv.Conv2d(64, 32, 3, padding=1, activation="relu").cuda()
     plain.load_state_dict(layer.state_dict())
     dx, db = torch.autograd.grad(y.float().sum(), (x, layer.bias))
@@ -257,4 +278,9 @@ def test_refusals_of_the_c_abi():
         for args, want in (((capi.F32, p, 0, 1, 8, p, p), capi.ERR_UNSUPPORTED), ((capi.F16, None, 0, 1, 8, p, p), bad), ((capi.F16, p, 0, 1, 8, None, p), bad),
                            ((capi.F16, p, 0, 1, 8, p, None), bad), ((capi.F16, p, 0, 0, 8, p, p), bad), ((capi.F16, p, 0, 1, 0, p, p), bad), ((capi.BF16, p, 7, 1, 8, p, p), bad),
                            ((capi.BF16, p + 1, 0, 1, 8, p, p), bad), ((capi.BF16, p, 0, 1 << 40, 8, p, p), capi.ERR_UNSUPPORTED)):
+            assert f(*args) == want, capi.last_error()
+    for f in (lambda dt, a, n, bits: lib.winoconv_sign_pack(dt, a, n, bits, None), lambda dt, a, n, bits: lib.winoconv_sign_apply(dt, a, bits, n, p, None),
+              lambda dt, a, n, bits: lib.winoconv_sign_apply(dt, p, bits, n, a, None)):
+        for args, want in (((capi.F32, p, 8, p), capi.ERR_UNSUPPORTED), ((capi.F16, None, 8, p), bad), ((capi.F16, p, 8, None), bad), ((capi.F16, p, 0, p), bad),
+                           ((capi.F16, p + 2, 8, p), bad), ((capi.F16, p, 1 << 41, p), capi.ERR_UNSUPPORTED)):
             assert f(*args) == want, capi.last_error()
