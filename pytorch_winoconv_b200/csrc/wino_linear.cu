@@ -286,6 +286,9 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(tmem_slot));
   tmem = __shfl_sync(0xffffffffu, tmem, 0);
   grid_dependency_wait();
+  const int n = min(g.tile_rows, o.rows - row0);
+  RowEnd<T, WIDE> end;
+  end.early(o, row0, col0, lane, (int)part + warp * split, 8 * split, n);
 
   if (warp == 0) {
     int s = 0;
@@ -325,9 +328,6 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
     if (alive && elect_one()) umma_commit<false>(done, 0);
   }
   __syncwarp();
-  const int n = min(g.tile_rows, o.rows - row0);
-  RowEnd<T, WIDE> end;
-  end.early(o, row0, col0, lane, (int)part + warp * split, 8 * split, n);
   // sums to shared memory: [row][128 columns]
   const bool ok = mbar_wait_warp(done, 0, abort_word, err, ERR_DONE);
   grid_launch_dependents();
@@ -346,6 +346,11 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
     tc_fence_before();
   }
   __syncthreads();
+  if (warp == 2) {
+    tc_fence_after();
+    tmem_free<false>(tmem, tmem_cols);
+  }
+  __syncwarp();
   if (split > 1) cluster_sync_all();
   if (*abort_word == 0u) {
     end.run(o, row0, col0, lane, (int)part + warp * split, 8 * split, n, [&](int j, float (&v)[4]) {
@@ -361,12 +366,6 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   }
   __syncwarp();
   if (split > 1) cluster_sync_all();      // no CTA leaves while another reads its shared memory
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 2) {
-    tc_fence_after();
-    tmem_free<false>(tmem, tmem_cols);
-  }
 }
 
 // ---- row kernel ------------------------------------------------------------------------------------------------------
@@ -379,8 +378,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
 // the kernel before: 9.6 and 7.5 us.  From three rows on the products cost more than the set-up (10.5 us against 8.6).
 constexpr int ROW_THREADS = 256, ROW_FEATURES = 4, MOST_ROWS = 2;
 
-// Lane sums of V values: afterwards v[0] of a lane is the sum over the warp of value `lane / (32 / V)`, with bits reversed as the
-// halving leaves them (index_of).
+// Lane sums of V values by halving: afterwards v[0] of a lane is the sum over the warp of value lane / (32 / V).
 template <int V> __device__ __forceinline__ void sum_lanes(float (&v)[V], int lane) {
 #pragma unroll
   for (int n = V, d = 16; n > 1; n >>= 1, d >>= 1) {
@@ -467,7 +465,6 @@ __global__ void __launch_bounds__(ROW_THREADS, 3) row_kernel(const T *x, long lo
     }
   }
   sum_lanes<V>(v, lane);
-  // the value that the halving left here: its index has the lane's upper bits, first halving first
   constexpr int LANES = 32 / V;
   const int index = lane / LANES;
   if (lane % LANES == 0) part[warp][index] = v[0];
