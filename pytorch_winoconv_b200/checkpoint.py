@@ -20,14 +20,21 @@ from . import _backend
 __all__ = ["BLOCK", "pack", "unpack"]
 
 BLOCK = 32
+_native = None
+
+
+def _module():
+    global _native
+    _native = _backend.load()
+    return _native
 
 
 def pack(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(q, scale)`` of a float16 or bfloat16 tensor: ``q`` of x's shape in ``torch.float8_e4m3fn``, ``scale``
     ``[..., ceil(C / 32)]`` in ``torch.float8_e8m0fnu``, both contiguous.  Not differentiable."""
-    return _backend.load().e4m3_pack(x)
+    return (_native or _module()).e4m3_pack(x)
 
 
 def unpack(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values that :func:`pack` kept, in ``dtype`` (float16 or bfloat16)."""
-    return _backend.load().e4m3_unpack(q, scale, dtype)
+    return (_native or _module()).e4m3_unpack(q, scale, dtype)

@@ -18,7 +18,9 @@
 // cluster share the reduction; the parts are added up over distributed shared memory in the same order by every CTA, vectors of four
 // read from all peers at once (sending single values to the CTA that finishes a row instead took 17.5 us where this took 10.8: 509 x 1000 x
 // 1531).  Two CTAs to an SM where the ring fits twice.  24 x 4096 x 16384 (f16) 23.5 us, 5.7 TB/s of weights; 64 x 4096 x 4096 10.2 us
-// and 16 x 4096 x 4096 8.1 us, of which the launch, the first loads, the exchange and the end take about 5.
+// and 16 x 4096 x 4096 8.1 us, of which the launch, the first loads, the exchange and the end take about 5.  Of 256 x 4096 x 4096's 15.5 us
+// the steps take 6.2 (L2), the hand-over 1.4, the exchange 3.5 (128 KB an SM over distributed shared memory, 19 bytes a clock: as long with
+// the sums of four rows in flight) and the end 0.9.
 //
 // Roles: warp 0 TMA, warp 1 MMA issue; then all eight warps move the accumulator to shared memory and add up and store their share
 // of the rows.  Every mbarrier wait is bounded and reports through the error word.
