@@ -281,7 +281,8 @@ __global__ void __launch_bounds__(THREADS) pad_rows_kernel(const __grid_constant
 // ---- gradient through the activation ---------------------------------------------------------------------------------
 // A block takes a strip of 32 x V columns and a run of rows, eight rows at a time; every thread adds up its own V columns in
 // fp32, the eight sums of a column are added in order, and a second kernel adds the runs in order: no atomics, the same bits
-// every time.
+// every time.  dz is rounded to the layer's type because the tensor cores read it for both products (their results carry the square
+// root of two times a single rounding's error for it); the bias gradient is summed from the values before that rounding.
 constexpr int ROWS = 8;
 
 using act::F2;
