@@ -378,7 +378,11 @@ __global__ void __launch_bounds__(THREADS, 4) act_grad_kernel(const __grid_const
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) s += part[i][j * 32 + l];
-    if (col < a.cols) a.ws[(long long)blockIdx.y * a.cols + col] = s;
+    if (col >= a.cols) continue;
+    if (chunks > 1) a.ws[(long long)blockIdx.y * a.cols + col] = s;
+    else if (a.dbias_dtype == WINOCONV_F32) ((float *)a.dbias)[col] = s;      // one run: nothing left to add
+    else if (a.dbias_dtype == WINOCONV_F16) Elem<__half>::store((__half *)a.dbias + col, s);
+    else Elem<__nv_bfloat16>::store((__nv_bfloat16 *)a.dbias + col, s);
   }
 }
 
@@ -450,7 +454,7 @@ template <typename T> cudaError_t act_grad(const ActGrad &a, cudaStream_t s) {
     }
   }
   const cudaError_t e = launch(kern, dim3((unsigned)((a.cols + 32 * v - 1) / (32 * v)), (unsigned)chunks), s, a, chunks);
-  if (e != cudaSuccess || !a.dbias) return e;
+  if (e != cudaSuccess || !a.dbias || chunks == 1) return e;
   const unsigned n = (unsigned)((a.cols + 31) / 32);
   if (a.dbias_dtype == WINOCONV_F32) return launch(column_sum_kernel<float>, n, s, a.ws, (float *)a.dbias, a.cols, chunks);
   if (a.dbias_dtype == WINOCONV_F16) return launch(column_sum_kernel<__half>, n, s, a.ws, (__half *)a.dbias, a.cols, chunks);

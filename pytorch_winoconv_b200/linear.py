@@ -74,6 +74,9 @@ class Linear(nn.Linear):
     Extra keyword arguments, as for ``conv.Conv2d``: ``compute_dtype`` (default ``torch.float16``; ``None`` keeps the input's
     type, which must then be a 16-bit one) is the type of the operands and the result; ``activation``; ``checkpoint``
     (``None`` / ``"e4m3"``).  ``forward`` takes the residual as a second argument.
+
+    Parameters of the compute type are read as they lie; float32 ones, a training loop's master copies, are rounded on every
+    call and get float32 gradients.  For serving, keep them in the compute type: ``layer.to(layer.compute_dtype)``.
     """
 
     def __init__(self, in_features, out_features, bias=True, device=None, dtype=None, *,
