@@ -105,9 +105,28 @@ winoconv_linear_desc_t describe(int64_t rows, int64_t k, int64_t n, at::ScalarTy
   return d;
 }
 
-// What a layer keeps for its backward pass: x and z, or their eight bits with the scales.
+// What a layer keeps for its backward pass: x and z, or one buffer with their eight bits and the scales.
 struct Kept {
-  at::Tensor x, x_scale, z, z_scale;
+  at::Tensor x, z, packed;
+};
+// Where the parts lie in that buffer, each on 16 bytes (sizes as kept; a part that is not kept has none).
+struct PackedAt {
+  int64_t x = 0, x_scale = 0, z = 0, z_scale = 0, bytes = 0;
+  PackedAt(int64_t rows, int64_t k, int64_t n, bool keep_x, bool keep_z) {
+    auto take = [&](int64_t b) {
+      const int64_t at = bytes;
+      bytes += (b + 15) / 16 * 16;
+      return at;
+    };
+    if (keep_x) {
+      x = take(rows * k);
+      x_scale = take(rows * ((k + 31) / 32));
+    }
+    if (keep_z) {
+      z = take(rows * n);
+      z_scale = take(rows * ((n + 31) / 32));
+    }
+  }
 };
 
 at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tensor &bias, const at::Tensor &residual, int act, bool pack, bool keep_x,
@@ -123,18 +142,18 @@ at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tens
     sizes.back() = n;
     y = at::empty(sizes, plain(x));
   }
-  const bool z = kept && keep_z;
-  if (kept && keep_x) {
-    if (pack) std::tie(kept->x, kept->x_scale) = e4m3_pack(x2);
-    else kept->x = x;
+  const bool z = kept && keep_z, z8 = z && pack;
+  const PackedAt lies(rows, k, n, kept && pack && keep_x, z8);
+  uint8_t *packed = nullptr;
+  if (kept && pack) {
+    kept->packed = at::empty({lies.bytes}, plain(x).dtype(at::kByte));
+    packed = (uint8_t *)kept->packed.data_ptr();
   }
-  if (z) {
-    kept->z = at::empty({rows, n}, pack ? plain(x).dtype(at::kFloat8_e4m3fn) : plain(x));
-    if (pack) kept->z_scale = at::empty({rows, (n + 31) / 32}, plain(x).dtype(at::kFloat8_e8m0fnu));
-  }
+  if (kept && keep_x && !pack) kept->x = x;
+  if (z && !pack) kept->z = at::empty({rows, n}, plain(x));
   if (rows == 0) return y;
   winoconv_linear_desc_t d = describe(rows, k, n, type, act);
-  const bool anywhere = rows <= 2 && !(z && pack);      // one or two rows are read as they lie
+  const bool anywhere = rows <= 2 && !z8;      // one or two rows are read as they lie
   Scratch scratch(d.dtype, x);
   Mat xm, wm;
   scratch.operand(x2, &xm, anywhere);
@@ -147,15 +166,19 @@ at::Tensor forward(const at::Tensor &x, const at::Tensor &weight, const at::Tens
   d.w_stride = wm.ld;
   if (r.defined() && rows > 1) d.residual_stride = row_stride(r);
   check_abi(winoconv_linear_forward(&d, xm.p, wm.p, b.defined() ? b.data_ptr() : nullptr, r.defined() ? r.data_ptr() : nullptr, y.data_ptr(),
-                                    z && !pack ? kept->z.data_ptr() : nullptr, z && pack ? kept->z.data_ptr() : nullptr,
-                                    z && pack ? kept->z_scale.data_ptr() : nullptr, stream_of()),
+                                    z && !pack ? kept->z.data_ptr() : nullptr, z8 ? packed + lies.z : nullptr, z8 ? packed + lies.z_scale : nullptr, stream_of()),
             "winoconv_linear_forward");
+  if (kept && keep_x && pack) {
+    const at::Tensor xr = with_rows(x2);
+    check_abi(winoconv_e4m3_pack(d.dtype, xr.data_ptr(), rows > 1 ? row_stride(xr) : 0, rows, (int32_t)k, packed + lies.x, packed + lies.x_scale, stream_of()),
+              "winoconv_e4m3_pack");
+  }
   return y;
 }
 
 struct LinearFn : public torch::autograd::Function<LinearFn> {
   // what the node remembers beside tensors, in one list of numbers: these, then the sizes of x
-  enum { X_TYPE, W_TYPE, B_TYPE, ACT, PACK, HAS_BIAS, HAS_RESIDUAL, OUT, IN, SIZES };
+  enum { X_TYPE, W_TYPE, B_TYPE, ACT, PACK, HAS_BIAS, HAS_RESIDUAL, KEEPS_X, KEEPS_Z, OUT, IN, SIZES };
 
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias,
                             const std::optional<at::Tensor> &residual, int64_t act, bool pack) {
@@ -167,9 +190,9 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
       y = ::forward(x, weight, bias ? *bias : at::Tensor(), residual ? *residual : at::Tensor(), (int)act, pack, nw,
                     act != WINOCONV_ACT_NONE && (nx || nw || nb), &kept);
     }
-    ctx->save_for_backward({kept.x, kept.x_scale, kept.z, kept.z_scale, nx ? weight : at::Tensor()});
+    ctx->save_for_backward({kept.x, kept.z, kept.packed, nx ? weight : at::Tensor()});
     std::vector<int64_t> layer{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(), bias ? (int64_t)bias->scalar_type() : -1, act, pack,
-                               bias.has_value(), residual.has_value(), weight.size(0), weight.size(1)};
+                               bias.has_value(), residual.has_value(), nw, act != WINOCONV_ACT_NONE && (nx || nw || nb), weight.size(0), weight.size(1)};
     layer.insert(layer.end(), x.sizes().begin(), x.sizes().end());
     ctx->saved_data["layer"] = std::move(layer);
     return y;
@@ -181,7 +204,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     at::AutoDispatchBelowADInplaceOrView no_graph;
     auto saved = ctx->get_saved_variables();
     const auto layer = ctx->saved_data["layer"].toIntVector();
-    for (int i = layer[PACK] ? 0 : 1; i < 4; ++i)      // dense, unless a hook on saved tensors has laid them out anew
+    for (int i = 1; i < 3; ++i)      // dense, unless a hook on saved tensors has laid them out anew
       if (saved[i].defined()) saved[i] = saved[i].contiguous();
     const auto type = (at::ScalarType)layer[X_TYPE], w_type = (at::ScalarType)layer[W_TYPE];
     const int act = (int)layer[ACT];
@@ -210,6 +233,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     }
     winoconv_linear_desc_t d = describe(rows, k, n, type, act);
     void *stream = stream_of();
+    const PackedAt lies(rows, k, n, pack && layer[KEEPS_X], pack && layer[KEEPS_Z]);
+    const uint8_t *packed = saved[2].defined() ? (const uint8_t *)saved[2].data_ptr() : nullptr;
     Scratch scratch(d.dtype, gy);
     Mat dz{g.data_ptr(), row_stride(g)}, w, x;
     // without an activation dz is gy as it lies, or a copy on 16 bytes
@@ -221,7 +246,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
       check_abi(winoconv_linear_backward_ws(&d, &ws_bytes), "winoconv_linear_backward_ws");
       ws_at = scratch.take((int64_t)ws_bytes);
     }
-    if (nx) scratch.operand(saved[4], &w);
+    if (nx) scratch.operand(saved[3], &w);
     if (nw) {
       if (pack) x_at = scratch.take(rows * round8(k) * 2);
       else scratch.operand(as_rows(saved[0], k), &x);
@@ -229,8 +254,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     scratch.allocate();
     if (write || nb) {
       if (write) dz = {scratch.pointer(dz_at), round8(n)};
-      check_abi(winoconv_linear_backward_activation(&d, g.data_ptr(), rows > 1 ? row_stride(g) : 0, slope && !pack ? saved[2].data_ptr() : nullptr,
-                                                    slope && pack ? saved[2].data_ptr() : nullptr, slope && pack ? saved[3].data_ptr() : nullptr,
+      check_abi(winoconv_linear_backward_activation(&d, g.data_ptr(), rows > 1 ? row_stride(g) : 0, slope && !pack ? saved[1].data_ptr() : nullptr,
+                                                    slope && pack ? packed + lies.z : nullptr, slope && pack ? packed + lies.z_scale : nullptr,
                                                     write ? dz.p : nullptr, write ? dz.ld : 0, nb ? db.data_ptr() : nullptr, nb ? code_of(db.scalar_type()) : 0,
                                                     nb ? scratch.pointer(ws_at) : nullptr, ws_bytes, stream),
                 "winoconv_linear_backward_activation");
@@ -242,7 +267,7 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     if (nw) {
       if (pack) {
         x = {scratch.pointer(x_at), round8(k)};
-        check_abi(winoconv_e4m3_unpack(d.dtype, saved[0].data_ptr(), saved[1].data_ptr(), rows, (int32_t)k, x.p, x.ld, stream), "winoconv_e4m3_unpack");
+        check_abi(winoconv_e4m3_unpack(d.dtype, packed + lies.x, packed + lies.x_scale, rows, (int32_t)k, x.p, x.ld, stream), "winoconv_e4m3_unpack");
       }
       d.x_stride = x.ld;
       check_abi(winoconv_linear_backward_weight(&d, dz.p, dz.ld, x.p, dw.data_ptr(), code_of(w_type), stream), "winoconv_linear_backward_weight");
