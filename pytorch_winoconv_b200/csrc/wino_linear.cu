@@ -52,7 +52,7 @@ enum ErrCode : unsigned { ERR_EMPTY = 0x601, ERR_FULL = 0x602, ERR_DONE = 0x603,
 
 // What the epilogues need of a problem.
 struct Out {
-  int rows, cols, act, layer, bias_f32, out_f32, wide;      // wide: rows of y, z and residual take vectors
+  int rows, cols, act, layer, bias_f32, out_f32, add, wide;      // add: to the f32 y that is there; wide: rows of y, z and residual take vectors
   const void *bias, *residual;
   void *y, *z;
   uint8_t *z8, *z8_scale;
@@ -166,7 +166,16 @@ __device__ __forceinline__ void finish4(const Out &o, int row, int col, int lane
       v[j] = y.lo() + residual[j]; v[j + 1] = y.hi() + residual[j + 1];
     }
   }
-  if (o.out_f32) store4<float, WIDE>((float *)o.y + row * o.y_stride + col, lane, cols, v);
+  if (o.out_f32) {
+    float *y = (float *)o.y + row * o.y_stride + col;
+    if (o.add) {
+      float before[4];
+      load4<float, WIDE>(y, lane, cols, before);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] += before[j];
+    }
+    store4<float, WIDE>(y, lane, cols, v);
+  }
   else store4<T, WIDE>((T *)o.y + row * o.y_stride + col, lane, cols, v);
 }
 
@@ -519,7 +528,7 @@ __device__ __forceinline__ void tile_at(const PairArgs &g, int t, int &rt, int &
 // 64 bytes of each of a warp's 32 rows (lane = row), turned in shared memory so that the stores of a row are contiguous.  EL:
 // bytes of an element; `rows` and `cols` are what is left of the matrix from here on.
 template <int EL>
-__device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16], uint8_t *dst, long long stride, int rows, int cols, int wide, int lane) {
+__device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16], uint8_t *dst, long long stride, int rows, int cols, int wide, int lane, int add = 0) {
   uint4 *mine = reinterpret_cast<uint4 *>(turn + lane * 64);
 #pragma unroll
   for (int i = 0; i < 4; ++i) mine[i ^ ((lane >> 1) & 3)] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
@@ -529,8 +538,16 @@ __device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i * 8 + (lane >> 2);
-      const uint4 v = *reinterpret_cast<const uint4 *>(turn + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-      if (r < rows && c * (16 / EL) < cols) *reinterpret_cast<uint4 *>(dst + r * stride + c * 16) = v;
+      uint4 v = *reinterpret_cast<const uint4 *>(turn + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+      if (r < rows && c * (16 / EL) < cols) {
+        uint4 *to = reinterpret_cast<uint4 *>(dst + r * stride + c * 16);
+        if (EL == 4 && add) {
+          const float4 b = *reinterpret_cast<const float4 *>(to);
+          v = make_uint4(__float_as_uint(__uint_as_float(v.x) + b.x), __float_as_uint(__uint_as_float(v.y) + b.y),
+                         __float_as_uint(__uint_as_float(v.z) + b.z), __float_as_uint(__uint_as_float(v.w) + b.w));
+        }
+        *to = v;
+      }
     }
   } else {
     constexpr int PER = 64 / EL, RS = 32 / PER;      // elements of a row, rows a time
@@ -539,7 +556,11 @@ __device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16
       const uint8_t *src = turn + r * 64 + ((((c * EL) >> 4) ^ ((r >> 1) & 3)) << 4) + ((c * EL) & 15);
       if (c < cols) {
         if constexpr (EL == 2) *reinterpret_cast<uint16_t *>(dst + r * stride + c * 2) = *reinterpret_cast<const uint16_t *>(src);
-        else *reinterpret_cast<uint32_t *>(dst + r * stride + c * 4) = *reinterpret_cast<const uint32_t *>(src);
+        else {
+          float *to = reinterpret_cast<float *>(dst + r * stride + c * 4);
+          const float v = *reinterpret_cast<const float *>(src);
+          *to = add ? v + *to : v;
+        }
       }
     }
   }
@@ -754,7 +775,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(f[16 * h + i]);
-            store_rows<4>(turn, w, dst + h * 64, o.y_stride * 4, rows, cols - 16 * h, o.wide, lane);
+            store_rows<4>(turn, w, dst + h * 64, o.y_stride * 4, rows, cols - 16 * h, o.wide, lane, o.add);
           }
         } else {
 #pragma unroll
@@ -796,7 +817,7 @@ bool multiple(const void *p, long long stride, int el, int bytes) {
 
 Out out_of(const LinearProblem &p, int width) {      // width: columns of a vector access
   Out o;
-  o.rows = p.rows; o.cols = p.cols; o.act = p.act; o.layer = p.layer; o.bias_f32 = p.bias_f32; o.out_f32 = p.out_f32;
+  o.rows = p.rows; o.cols = p.cols; o.act = p.act; o.layer = p.layer; o.bias_f32 = p.bias_f32; o.out_f32 = p.out_f32; o.add = p.add;
   o.bias = p.bias; o.residual = p.residual; o.y = p.y; o.z = p.z; o.z8 = p.z8; o.z8_scale = p.z8_scale;
   o.residual_stride = p.residual_stride; o.y_stride = p.y_stride; o.z_stride = p.z_stride;
   const int el = p.out_f32 ? 4 : 2;
@@ -958,13 +979,32 @@ LinearPlan linear_plan(const LinearProblem &p) {
   return plan;
 }
 
-cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
+static cudaError_t launch_form(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
   *detail = "";
   if (plan.by_rows) return p.dtype == WINOCONV_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
   if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, plan.pair, enc, s, detail) : launch_pair<__nv_bfloat16>(p, plan.pair, enc, s, detail);
   return p.dtype == WINOCONV_F16 ? launch_cluster<__half>(p, plan, enc, s, detail) : launch_cluster<__nv_bfloat16>(p, plan, enc, s, detail);
+}
+
+// The tensor cores cut off what an fp32 accumulator has no place for, at every 16 values of the reduction: sums of one sign lose
+// 5e-5 of their value over 65536 values and 9e-4 over 2^20 (sums of both signs 1e-5 and 1.5e-4), which 16 bits do not show but f32 results
+// do.  These are added up over runs of 16384 values, a launch each (1e-5 and 3e-6 over any number).
+constexpr int RUN = 16384;
+cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
+  if (!p.out_f32 || p.red <= RUN) return launch_form(p, plan, s, detail);
+  cudaError_t e = cudaSuccess;
+  for (int k = 0; k < p.red && e == cudaSuccess; k += RUN) {
+    LinearProblem q = p;
+    q.red = std::min(RUN, p.red - k);
+    q.add = k > 0;
+    auto from = [&](const MatOperand &m) { return MatOperand{(const uint16_t *)m.ptr + (m.mn ? (long long)k * m.stride : (long long)k), m.stride, m.mn}; };
+    q.r = from(p.r);
+    q.c = from(p.c);
+    e = launch_form(q, linear_plan(q), s, detail);
+  }
+  return e;
 }
 
 cudaError_t read_and_clear_linear_error(cudaStream_t s, unsigned int *code) {

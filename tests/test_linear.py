@@ -416,6 +416,24 @@ def test_more_values_than_32_bits_count():
 
 
 @gpu
+@pytest.mark.parametrize("rows,k,n", [(40_000, 72, 130), (33_000, 1030, 515), (50_001, 31, 65)])
+def test_float_weight_gradients_of_many_rows(rows, k, n):
+    """Added up over runs of rows: exact where every sum is (below 2^24 of the smallest step), and without the drift of one long
+    chain where it is not: a run of 16384 rows is 1024 additions, each cuts off less than a step of 2^-23 of a sum that is half the
+    last one on average, so sums of one sign are within 1024 x 2^-24."""
+    x = ints((rows, k), 1, 4, 0.25, torch.float16)
+    gy = ints((rows, n), 2, 4, 2.0 ** -6, torch.float16)
+    w = torch.zeros(n, k, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(lin.linear(x, w), w, gy)
+    assert torch.equal(dw, (gy.double().t() @ x.double()).float())
+    x, gy = (torch.rand(rows, c, device="cuda", generator=torch.Generator(device="cuda").manual_seed(c)).half() for c in (k, n))
+    dw, = torch.autograd.grad(lin.linear(x, w), w, gy)
+    want = gy.double().t() @ x.double()
+    assert ((dw.double() - want).abs() <= want * 1024 * 2.0 ** -24).all()
+    assert capi.read_device_error() == 0
+
+
+@gpu
 def test_a_first_call_that_is_captured():
     """A fresh process whose first calls of the layer are in a capture, forward and backward: kernels are loaded and attributes set
     without a word to the stream, and the replay gives the eager values."""
