@@ -7,7 +7,8 @@ bits, so what comes back is held by float16 and bfloat16 without another roundin
 rounds up beyond the type's largest (65504 in float16) comes back as that largest.
 
 ``linear.Linear``, ``conv.Conv2d`` and ``conv.Conv3d`` use it with ``checkpoint="e4m3"`` (a convolution packs the channels of each
-pixel: fewer than 32 save less); :func:`pack` and :func:`unpack` are the operators themselves, for a program's own autograd functions.
+pixel: fewer than 32 save less); :func:`pack` and :func:`unpack` are the operators themselves, for a program's own autograd functions
+(calls that a tracer would record or that carry a forward-mode gradient are errors).
 """
 from __future__ import annotations
 

@@ -1,7 +1,9 @@
 #include "linear_module.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <vector>
 
@@ -278,8 +280,22 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
 
 }  // namespace
 
+void check_eager(const char *what, std::initializer_list<const at::Tensor *> tensors) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  bool recorded = torch::jit::tracer::isTracing();
+  if (Modes::any_modes_set())      // (a mode that only watches is no hindrance)
+    for (Key k : {Key::FAKE, Key::PROXY, Key::FUNCTIONAL}) recorded = recorded || Modes::get_mode(k).has_value();
+  TORCH_CHECK(!recorded, what, ": the call cannot be recorded by a tracer: run it eagerly, or capture it into a CUDA graph");
+  for (const at::Tensor *t : tensors)
+    TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, ": there is no forward-mode differentiation");
+}
+
 at::Tensor linear_call(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, const std::optional<at::Tensor> &residual,
                        int64_t act, bool pack) {
+  check_eager("linear", {&x, &weight});
+  if (bias) check_eager("linear", {&*bias});
+  if (residual) check_eager("linear", {&*residual});
   TORCH_CHECK(x.is_cuda(), "linear runs on CUDA devices only: there is no CPU path");
   TORCH_CHECK(is16(x), "linear: x must be float16 or bfloat16, got ", x.scalar_type());
   TORCH_CHECK(weight.dim() == 2, "linear: weight must be [out_features, in_features], got ", weight.sizes());
@@ -309,6 +325,7 @@ at::Tensor linear_call(const at::Tensor &x, const at::Tensor &weight, const std:
 }
 
 std::tuple<at::Tensor, at::Tensor> e4m3_pack(const at::Tensor &x_in) {
+  check_eager("checkpoint.pack", {&x_in});
   TORCH_CHECK(x_in.is_cuda(), "checkpoint.pack runs on CUDA devices only: there is no CPU path");
   TORCH_CHECK(is16(x_in), "checkpoint.pack: x must be float16 or bfloat16, got ", x_in.scalar_type());
   TORCH_CHECK(x_in.dim() >= 1 && x_in.size(-1) > 0, "checkpoint.pack: x must have a last dimension that is not empty, got ", x_in.sizes());
@@ -328,6 +345,7 @@ std::tuple<at::Tensor, at::Tensor> e4m3_pack(const at::Tensor &x_in) {
 }
 
 at::Tensor e4m3_unpack(const at::Tensor &q_in, const at::Tensor &scale_in, at::ScalarType type) {
+  check_eager("checkpoint.unpack", {&q_in, &scale_in});
   TORCH_CHECK(q_in.is_cuda() && scale_in.device() == q_in.device(), "checkpoint.unpack runs on CUDA devices only, q and scale on the same one");
   TORCH_CHECK(q_in.scalar_type() == at::kFloat8_e4m3fn && scale_in.scalar_type() == at::kFloat8_e8m0fnu,
               "checkpoint.unpack: q must be float8_e4m3fn and scale float8_e8m0fnu, got ", q_in.scalar_type(), " and ", scale_in.scalar_type());

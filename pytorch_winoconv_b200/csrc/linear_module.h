@@ -3,10 +3,16 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 #include <optional>
 #include <tuple>
 
 #include <torch/extension.h>
+
+// Raises where the call would be recorded (torch.jit.trace, make_fx, torch.export) or carries a forward-mode gradient: what is
+// launched here is seen neither by a tracer, to which the result would be an empty tensor, nor by forward-mode differentiation, to
+// which it would be a constant.
+void check_eager(const char *what, std::initializer_list<const at::Tensor *> tensors);
 
 // y = act(x weight^T + bias) + residual in x's type (f16 or bf16); act: winoconv_act_t.  weight and bias are of that type or f32
 // (the weight is then rounded once, the bias added as it is).  pack: what the backward pass needs of x and of the

@@ -16,7 +16,8 @@ give the same bits every time.
 
 The gradients are not differentiable again.  There is no CPU path and no library product.  Calls keep nothing but what autograd
 saves: they may run on several threads and streams and in captured graphs.  (As with every operator of torch, a backward pass can only
-be captured when no eager graph of the same parameters, built on another stream, is still alive: torch raises there.)
+be captured when no eager graph of the same parameters, built on another stream, is still alive: torch raises there.)  A call that a
+tracer would record (``torch.jit.trace``, ``make_fx``, ``torch.export``) or that carries a forward-mode gradient is an error.
 """
 from __future__ import annotations
 

@@ -284,3 +284,18 @@ def test_refusals_of_the_c_abi():
         for args, want in (((capi.F32, p, 8, p), capi.ERR_UNSUPPORTED), ((capi.F16, None, 8, p), bad), ((capi.F16, p, 8, None), bad), ((capi.F16, p, 0, p), bad),
                            ((capi.F16, p + 2, 8, p), bad), ((capi.F16, p, 1 << 41, p), capi.ERR_UNSUPPORTED)):
             assert f(*args) == want, capi.last_error()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_recorded_calls_and_forward_mode_are_refused(device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 40, device=device).half()
+    q, scale = torch.zeros(4, 40, device=device).to(torch.float8_e4m3fn), torch.zeros(4, 2, dtype=torch.uint8, device=device).view(torch.float8_e8m0fnu)
+    for call, args in ((lambda t: checkpoint.pack(t)[0].view(torch.uint8), (x,)), (lambda a, s: checkpoint.unpack(a, s), (q, scale))):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(call, args)
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            make_fx(call)(*args)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            checkpoint.pack(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))

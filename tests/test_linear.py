@@ -659,3 +659,27 @@ def test_the_c_abi_reports_a_missing_device():
     p = 1 << 20
     d = capi.LinearDesc(rows=4, in_features=16, out_features=24, dtype=capi.F16)
     assert capi.lib().winoconv_linear_forward(ctypes.byref(d), p, p, None, None, p, None, None, None, None) == capi.ERR_NO_DEVICE
+
+
+# ---- calls that would be recorded or differentiated as something else ---------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_recorded_calls_and_forward_mode_are_refused(device):
+    """A tracer sees nothing of a layer but its empty output, and a forward-mode gradient would be lost: both are errors, on every device."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w, b, r = (ints(s, i, 4, 0.25, torch.float16, device) for i, s in enumerate([(4, 40), (24, 40), (24,), (4, 24)]))
+    layer = lin.Linear(40, 24, device=device, dtype=torch.float16)
+    for leaves in (False, True):
+        for p in layer.parameters():
+            p.requires_grad_(leaves)
+        for call in (lambda t: lin.linear(t, w, b, activation="gelu"), layer):
+            with pytest.raises(RuntimeError, match="cannot be recorded"):
+                torch.jit.trace(call, x)
+            with pytest.raises(RuntimeError, match="cannot be recorded"):
+                make_fx(call)(x)
+    for i, t in enumerate((x, w, b, r)):
+        with torch.autograd.forward_ad.dual_level():
+            args = [torch.autograd.forward_ad.make_dual(t, torch.ones_like(t)) if j == i else s for j, s in enumerate((x, w, b, r))]
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                lin.linear(*args)
+    if device == "cuda":      # and nothing of it lasts
+        assert torch.equal(lin.linear(x, w, b, r), forward64(x, w, b, r, None)[1].half())
