@@ -272,6 +272,8 @@ at::Tensor ConvRunner::run(Entry &e, const at::Tensor &x, const at::Tensor &weig
 }
 
 std::optional<at::Tensor> ConvRunner::forward(const at::Tensor &x, const at::Tensor &weight, const std::optional<at::Tensor> &bias, bool training) {
+  check_eager("convolution", {&x, &weight});
+  if (bias) check_eager("convolution", {&*bias});
   if (!x.is_cuda() || x.dim() != nd_ + 2 || weight.dim() != nd_ + 2 || !weight.is_cuda() || weight.get_device() != x.get_device() ||
       x.size(1) != weight.size(1) || x.numel() == 0 || code_of(weight.scalar_type()) < 0 ||
       (bias && (!bias->is_cuda() || bias->get_device() != x.get_device() || bias->numel() != weight.size(0))))
@@ -424,6 +426,8 @@ std::vector<std::tuple<std::vector<int64_t>, int64_t, int64_t, at::Tensor, int64
 
 std::optional<at::Tensor> conv_call(const at::Tensor &x_in, const at::Tensor &weight_in, const std::optional<at::Tensor> &bias,
                                     std::vector<int64_t> stride, std::vector<int64_t> padding, int64_t compute, bool out_f32, int64_t tile_m) {
+  check_eager("convolution", {&x_in, &weight_in});
+  if (bias) check_eager("convolution", {&*bias});
   const int nd = (int)x_in.dim() - 2;
   if (!x_in.is_cuda() || (nd != 2 && nd != 3) || weight_in.dim() != nd + 2 || x_in.size(1) != weight_in.size(1) || x_in.numel() == 0 ||
       weight_in.numel() == 0 || (int)stride.size() != nd || (int)padding.size() != nd || (bias && bias->numel() != weight_in.size(0)))

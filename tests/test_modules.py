@@ -609,3 +609,37 @@ def test_a_graph_keeps_the_filters_it_was_captured_with():
         assert _rel(y, o + b + 1) < _ONE_ROUNDING[torch.float16]
         assert _rel(z, _by_torch(m, x)) < _ONE_ROUNDING[torch.float16]
         del spoil
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_recorded_calls_and_forward_mode_are_refused(device):
+    """A tracer sees nothing of a layer but its empty output, and a forward-mode gradient would be lost: both are errors, on every device."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    ad = torch.autograd.forward_ad
+    for cls, shape in ((wconv.Conv2d, (1, 4, 8, 8)), (wconv.Conv3d, (1, 4, 5, 6, 7))):
+        for kw in ({}, {"checkpoint": "e4m3", "activation": "relu"}, {"compute_dtype": torch.float32}):
+            layer = cls(4, 8, 3, **kw).to(device)
+            x = torch.randn(shape, device=device)
+            for leaves in (True, False):
+                for p in layer.parameters():
+                    p.requires_grad_(leaves)
+                with pytest.raises(RuntimeError, match="cannot be recorded"):
+                    torch.jit.trace(layer, x)
+                with pytest.raises(RuntimeError, match="cannot be recorded"):
+                    make_fx(layer)(x)
+            with ad.dual_level():
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    layer(ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.gpu
+def test_recorded_calls_and_forward_mode_are_refused_by_the_functions():
+    from pytorch_winoconv_b200 import dwm, matrix_conv, matrix_conv3d
+    ad = torch.autograd.forward_ad
+    x, w = torch.randn(1, 4, 8, 8, device="cuda"), torch.randn(8, 4, 3, 3, device="cuda")
+    for call, a, b in ((matrix_conv.conv16, x, w), (dwm.dwm2d, x, w), (matrix_conv3d.conv16, x[:, :, None].repeat(1, 1, 5, 1, 1), w[:, :, None].repeat(1, 1, 3, 1, 1))):
+        with pytest.raises(RuntimeError, match="cannot be recorded"):
+            torch.jit.trace(lambda t: call(t, b), a)
+        with ad.dual_level():
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(a, ad.make_dual(b, torch.ones_like(b)))
