@@ -63,9 +63,10 @@ template <typename T> __device__ __forceinline__ float within(float v) {      //
 
 namespace act {
 
-// The smooth activations are built from the hardware's 2^x and 1/x (each good to a few 2^-23 relative), far below the 2^-9 or
-// 2^-12 that rounding a result to 16 bits costs, and work on two values an instruction: a kernel that passes over memory at
-// 6.5 TB/s has about 20 instructions a value to spend.
+// The smooth activations are built from the hardware's 2^x and 1/x (each good to a few 2^-23 relative) and keep a relative error of
+// 2^-18 plus what the argument of the exponential loses (2^-23 of its size, which is below 16 for results that f16 holds and below 128
+// for bf16's; results below 2^-126 are 0): far below the 2^-9 or 2^-12 that rounding a result to 16 bits costs.  They work on two values
+// an instruction: a kernel that passes over memory at 6.5 TB/s has about 20 instructions a value to spend.
 struct F2 {      // two fp32 values
   uint64_t v;
   F2() = default;
@@ -96,16 +97,21 @@ __device__ __forceinline__ F2 square256(F2 z) { return each(z * z, [](float t) {
 __device__ __forceinline__ F2 gelu_sigmoid(F2 z, F2 z2) {
   return recip(exp2_fast(z * fma2(z2, F2(-2.f * LOG2E * GELU_C * GELU_A), F2(-2.f * LOG2E * GELU_C))) + F2(1.f));
 }
-// The normal distribution's integral, and its density, with one exponential: erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) with
-// t = 1 / (1 + p x) for x >= 0 (Abramowitz and Stegun, formula 7.1.26: within 1.5e-7 of erf).
+// The normal distribution's integral, and its density, with one exponential.  For x >= 0 the integral from x on is exp(-x^2 / 2) g(x),
+// where g falls from 1/2 like 1 / (x sqrt(2 pi)): here a polynomial in t = 1 / (1 + p x) without a constant term, p and its
+// coefficients fitted (linear program on 2700 points of 0..13.5) for the smallest relative error, 5.3e-7; 1.5e-6 with fp32 steps up to
+// x = 8, 4e-6 up to 13.2, where the exponential ends.  The relative error is what counts: GELU of a far negative z is z times the tail
+// (a tail that is good to 1e-7 absolutely is off by 5e-4 of its value at -4 and 4e-3 at -6).
 __device__ __forceinline__ F2 normal(F2 z, F2 &density) {
-  const F2 x = each(z * F2(0.7071067811865476f), [](float t) { return fabsf(t); });
-  const F2 e = exp2_fast(x * x * F2(-LOG2E)), t = recip(fma2(x, F2(0.3275911f), F2(1.f)));
-  F2 p = fma2(t, F2(1.061405429f), F2(-1.453152027f));
-  p = fma2(t, p, F2(1.421413741f));
-  p = fma2(t, p, F2(-0.284496736f));
-  p = fma2(t, p, F2(0.254829592f));
-  const F2 tail = p * t * (e * F2(0.5f)), body = fma2(tail, F2(-1.f), F2(1.f));
+  const F2 x = each(z, [](float t) { return fabsf(t); });
+  const F2 e = exp2_fast(z * z * F2(-0.5f * LOG2E)), t = recip(fma2(x, F2(0.26389465f), F2(1.f)));
+  F2 p = fma2(t, F2(-0.06941466f), F2(0.20421680f));
+  p = fma2(t, p, F2(-0.07724253f));
+  p = fma2(t, p, F2(0.14928270f));
+  p = fma2(t, p, F2(0.08021010f));
+  p = fma2(t, p, F2(0.10781857f));
+  p = fma2(t, p, F2(0.10512876f));
+  const F2 tail = p * t * e, body = fma2(tail, F2(-1.f), F2(1.f));
   density = e * F2(0.3989422804014327f);
   return F2(z.lo() < 0.f ? tail.lo() : body.lo(), z.hi() < 0.f ? tail.hi() : body.hi());
 }

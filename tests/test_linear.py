@@ -683,3 +683,47 @@ def test_recorded_calls_and_forward_mode_are_refused(device):
                 lin.linear(*args)
     if device == "cuda":      # and nothing of it lasts
         assert torch.equal(lin.linear(x, w, b, r), forward64(x, w, b, r, None)[1].half())
+
+
+# ---- how good an activation is, relative to its value --------------------------------------------------------------------
+def smooth64(z, act):
+    """Value, slope, the size of what the slope is a sum of, and the relative error that fp32 leaves of either.
+
+    The exponential's argument t carries about three roundings of 2^-24 relative each (eight with the cubic), which are as many of |t|
+    relative to the result; 2^-18 stands for the rest: 2^x and 1/x to a few 2^-22, a fitted tail to 2^-20, some products."""
+    if act == "gelu":
+        tail, density = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5), torch.exp(-z * z / 2) * (2 * torch.pi) ** -0.5
+        return z * tail, tail + z * density, tail + (z * density).abs(), 2.0 ** -18 + z * z * 2.0 ** -23
+    if act == "gelu_tanh":
+        c, a = 2 * (2 / torch.pi) ** 0.5, 0.044715
+        t, dt = c * (z + a * z ** 3), c * (1 + 3 * a * z * z)
+        s, off = torch.sigmoid(t), 2.0 ** -18 + t.abs() * 2.0 ** -21
+    else:
+        t, dt, s, off = z, 1.0, torch.sigmoid(z), 2.0 ** -18 + z.abs() * 2.0 ** -22
+    bend = z * s * torch.sigmoid(-t) * dt
+    return z * s, s + bend, s + bend.abs(), off
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_keep_their_relative_precision(act, dtype):
+    """Every value of the type up to 30 as a pre-activation, through each of the kernels: the far side of zero too is good to half a step
+    of the result (and to 2^-126, below which the hardware's 2^x is zero)."""
+    z = torch.arange(65536, dtype=torch.int32).to(torch.int16).cuda().view(dtype)
+    z = z[z.abs() <= 30][:, None].contiguous()      # (NaN compares as false)
+    one = torch.ones(1, 1, dtype=dtype, device="cuda")
+    zd = z.double()
+    y, slope, size, off = smooth64(zd, act)
+    floor = (1 + zd.abs() + zd.abs() ** 3) * 2.0 ** -126
+    check(lin.linear(z, one, activation=act), y, act, dtype, extra=y.abs() * off + floor)                                    # clusters
+    check(lin.linear(one, z, activation=act), y.t(), act, dtype, extra=(y.abs() * off + floor).t())                          # one row
+    many = lin.linear(z, one.expand(264, 1).contiguous(), activation=act)                                                    # pairs
+    check(many[:, :1], y, act, dtype, extra=y.abs() * off + floor)
+    assert torch.equal(many, many[:, :1].expand_as(many))
+    for cols in (1, 8):      # the gradient's pass by single values and by vectors; each of eight equal columns gives an eighth, rounded by itself
+        leaf = z.clone().requires_grad_()
+        w = torch.ones(cols, 1, dtype=dtype, device="cuda")
+        dx, = torch.autograd.grad(lin.linear(leaf, w, activation=act), leaf, torch.full((len(z), cols), 1 / cols, dtype=dtype, device="cuda"))
+        check(dx, slope, act, dtype, extra=size * off + floor + (0 if cols == 1 else 8 * half_step(slope / 8, dtype)))
+    assert capi.read_device_error() == 0
