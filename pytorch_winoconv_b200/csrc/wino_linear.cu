@@ -52,7 +52,7 @@ enum ErrCode : unsigned { ERR_EMPTY = 0x601, ERR_FULL = 0x602, ERR_DONE = 0x603,
 
 // What the epilogues need of a problem.
 struct Out {
-  int rows, cols, act, layer, bias_f32, out_f32, add, wide;      // add: to the f32 y that is there; wide: rows of y, z and residual take vectors
+  int rows, cols, act, layer, bias_f32, out_f32, wide;      // wide: rows of y, z and residual take vectors
   const void *bias, *residual;
   void *y, *z;
   uint8_t *z8, *z8_scale;
@@ -96,6 +96,28 @@ __device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
 // 8 KB apart, groups of eight reduction steps 1 KB apart; K-major: groups of eight rows 1 KB apart.
 __device__ __forceinline__ uint32_t operand_lo(uint32_t saddr, int mn) { return desc_lo(saddr, mn ? 8192u : 16u); }
 __device__ __forceinline__ uint32_t operand_step(int mn) { return mn ? 128u : 2u; }
+
+// Long reductions.  The tensor cores cut products and sum off about two bits below the sum's last place, at every 16 values: sums of
+// one sign lose 1.7 x 2^-24 of their value for each 16 (the worst of constant columns: 3.0; sums of both signs lose nothing that is seen),
+// 1e-4 over 16384.  So an accumulator takes a run of the reduction at most, and the runs are added up in fp32, rounded to nearest, in
+// tensor memory: the first run's accumulator holds the sum, the others' take turns in a second one.  A run is as long as half a step of the
+// result's type allows: at worst 4.6e-5 in f32 results, 1.8e-4 in f16 (half a step: 2.4e-4 to 4.9e-4), 7.3e-4 in bf16 (2.0e-3 to
+// 3.9e-3).  No wait lasts longer than a run, however long the reduction.
+constexpr int RUN_F32 = 4096 / BK, RUN_F16 = 16384 / BK, RUN_BF16 = 65536 / BK;      // steps
+int steps_of_a_run(const LinearProblem &p) { return p.out_f32 ? RUN_F32 : p.dtype == WINOCONV_F16 ? RUN_F16 : RUN_BF16; }
+// The step at which run `r` of `runs` starts.
+__device__ __forceinline__ int run_start(int steps, int r, int runs) { return (int)((long long)steps * r / runs); }
+// 32 lanes x 32 columns of `sum` plus those of `run`.
+__device__ __forceinline__ void add_run(uint32_t sum, uint32_t run) {
+  uint32_t a[32], b[32];
+  tmem_ld_x32(sum, a);
+  tmem_ld_x32(run, b);
+  tmem_wait_ld_x32(a);
+  tmem_wait_ld_x32(b);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) + __uint_as_float(b[i]));
+  tmem_st_x32(sum, a);
+}
 
 // A lane's four columns of a row in the cluster kernel's epilogue.  WIDE: neighbours, moved as one vector; else 32 apart, so that a
 // warp's accesses of single values are contiguous.
@@ -166,16 +188,7 @@ __device__ __forceinline__ void finish4(const Out &o, int row, int col, int lane
       v[j] = y.lo() + residual[j]; v[j + 1] = y.hi() + residual[j + 1];
     }
   }
-  if (o.out_f32) {
-    float *y = (float *)o.y + row * o.y_stride + col;
-    if (o.add) {
-      float before[4];
-      load4<float, WIDE>(y, lane, cols, before);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += before[j];
-    }
-    store4<float, WIDE>(y, lane, cols, v);
-  }
+  if (o.out_f32) store4<float, WIDE>((float *)o.y + row * o.y_stride + col, lane, cols, v);
   else store4<T, WIDE>((T *)o.y + row * o.y_stride + col, lane, cols, v);
 }
 
@@ -247,7 +260,7 @@ template <int S, bool WIDE> __device__ __forceinline__ void add_parts(uint32_t s
 }
 
 struct ClusterArgs {
-  int n_steps, n_rt, tile_rows, stages, r_mn, c_mn;
+  int n_steps, run, n_rt, tile_rows, stages, r_mn, c_mn;
   uint32_t idesc;
 };
 
@@ -264,10 +277,10 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   uint8_t *base_ptr = smem_raw + (base - raw);
   const uint32_t stage_bytes = (uint32_t)(C_BYTES + g.tile_rows * BK * 2);
   const uint32_t ring = max((uint32_t)g.stages * stage_bytes, (uint32_t)(g.tile_rows * BC * 4));      // or the sums, whichever is longer
-  const uint32_t bars = base + ring;      // full[8] empty[8] done
+  const uint32_t bars = base + ring;      // full[8] empty[8] done run_full run_free
   auto full = [&](int i) { return bars + 8u * i; };
   auto empty = [&](int i) { return bars + 64u + 8u * i; };
-  const uint32_t done = bars + 128u, tmem_slot = bars + 196u;
+  const uint32_t done = bars + 128u, run_full = bars + 136u, run_free = bars + 144u, tmem_slot = bars + 196u;
   volatile unsigned *abort_word = reinterpret_cast<volatile unsigned *>(base_ptr + ring + 192);
   unsigned *err = &g_linear_error;
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -276,8 +289,10 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   const int tile = (int)blockIdx.x / split, ct = tile / g.n_rt, rt = tile - ct * g.n_rt;      // CTAs in flight share columns: the weights are read once
   const int row0 = rt * g.tile_rows, col0 = ct * BC;
   const int k0 = (int)((long long)g.n_steps * part / split), k1 = (int)((long long)g.n_steps * (part + 1) / split);
-  uint32_t tmem_cols = 32;
-  while (tmem_cols < (uint32_t)g.tile_rows) tmem_cols *= 2;
+  const int steps = k1 - k0, runs = (steps + g.run - 1) / g.run;
+  uint32_t acc_cols = 32;
+  while (acc_cols < (uint32_t)g.tile_rows) acc_cols *= 2;
+  const uint32_t tmem_cols = runs > 1 ? 2u * acc_cols : acc_cols;
 
   if (warp == 1 && lane == 0) prefetch_map(&map_r);
   // The first stages of C (the weights) are sent for while this kernel sets itself up and the one before it ends; into L2 only,
@@ -285,7 +300,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   if (warp == 3 && lane < g.stages && k0 + lane < k1) prefetch_operand(&map_c, g.c_mn, col0, BC, (k0 + lane) * BK);
   if (warp == 0) {
     if (lane < 8) { mbar_init(full(lane), 1); mbar_init(empty(lane), 1); }
-    else if (lane == 8) mbar_init(done, 1);
+    else if (lane == 8) { mbar_init(done, 1); mbar_init(run_full, 1); mbar_init(run_free, CLUSTER_THREADS / 32 - 2); }
     else if (lane == 9) *abort_word = 0u;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -319,24 +334,48 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
       while (clock64() - start < 2000000LL) { }
     }
   } else if (warp == 1) {
-    int s = 0;
+    int s = 0, k = k0;
     uint32_t ph = 0;
     bool alive = true;
-    for (int k = k0; k < k1; ++k) {
-      if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
-      tc_fence_after();
-      const uint32_t st = base + (uint32_t)s * stage_bytes;
-      const uint32_t a = operand_lo(st, g.c_mn), b = operand_lo(st + C_BYTES, g.r_mn), hi = desc_hi(1024, 2);
-      if (elect_one()) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          umma<false, false>(tmem, a + (uint32_t)j * operand_step(g.c_mn), hi, b + (uint32_t)j * operand_step(g.r_mn), hi, g.idesc, (k > k0 || j > 0) ? 1u : 0u);
-        umma_commit<false>(empty(s), 0);
+    for (int run = 0; run < runs && alive; ++run) {
+      if (run > 0) {
+        if (!mbar_wait_warp(run_free, (uint32_t)(run - 1) & 1u, abort_word, err, ERR_ACC_EMPTY)) { alive = false; break; }
+        tc_fence_after();
       }
+      const int first = k, last = k0 + run_start(steps, run + 1, runs);
+      const uint32_t d = run > 0 ? tmem + acc_cols : tmem;
+      for (; k < last; ++k) {
+        if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
+        tc_fence_after();
+        const uint32_t st = base + (uint32_t)s * stage_bytes;
+        const uint32_t a = operand_lo(st, g.c_mn), b = operand_lo(st + C_BYTES, g.r_mn), hi = desc_hi(1024, 2);
+        if (elect_one()) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            umma<false, false>(d, a + (uint32_t)j * operand_step(g.c_mn), hi, b + (uint32_t)j * operand_step(g.r_mn), hi, g.idesc, (k > first || j > 0) ? 1u : 0u);
+          umma_commit<false>(empty(s), 0);
+        }
+        __syncwarp();
+        if (++s == g.stages) { s = 0; ph ^= 1u; }
+      }
+      if (alive && elect_one()) umma_commit<false>(run + 1 < runs ? run_full : done, 0);
       __syncwarp();
-      if (++s == g.stages) { s = 0; ph ^= 1u; }
     }
-    if (alive && elect_one()) umma_commit<false>(done, 0);
+  } else {
+    // every run but the last: the second accumulator into the first (all six warps answer, so that none falls two runs behind)
+    for (int run = 0; run + 1 < runs; ++run) {
+      if (!mbar_wait_warp(run_full, (uint32_t)run & 1u, abort_word, err, ERR_ACC_FULL)) break;
+      tc_fence_after();
+      if (run > 0 && warp >= 4) {
+        const uint32_t at = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+#pragma unroll 1
+        for (int c = 0; c < n; c += 32) add_run(at + (uint32_t)c, at + acc_cols + (uint32_t)c);
+        tmem_wait_st();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(run_free);
+    }
   }
   __syncwarp();
   // sums to shared memory: [row][128 columns]
@@ -350,6 +389,13 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
       uint32_t v[32];
       tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)c, v);
       tmem_wait_ld_x32(v);
+      if (runs > 1) {      // the last run's
+        uint32_t u[32];
+        tmem_ld_x32(tmem + ((uint32_t)(q * 32) << 16) + acc_cols + (uint32_t)c, u);
+        tmem_wait_ld_x32(u);
+#pragma unroll
+        for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(__uint_as_float(v[j]) + __uint_as_float(u[j]));
+      }
 #pragma unroll
       for (int j = 0; j < 32; ++j)
         if (c + j < n) sums[(c + j) * BC + q * 32 + lane] = __uint_as_float(v[j]);
@@ -513,7 +559,7 @@ template <int BN> struct PairTile {
 };
 
 struct PairArgs {
-  int n_steps, n_rt, n_ct, n_tiles, band, r_mn, c_mn;
+  int n_steps, runs, n_rt, n_ct, n_tiles, band, r_mn, c_mn;
   uint32_t idesc;
 };
 // Tiles are walked in bands of tile rows, column by column: the pairs at work at one time share few rows and few columns, which then
@@ -530,7 +576,7 @@ int band_of(int red) { return (int)std::min(16LL, std::max(8LL, 36000000LL / ((l
 // 64 bytes of each of a warp's 32 rows (lane = row), turned in shared memory so that the stores of a row are contiguous.  EL:
 // bytes of an element; `rows` and `cols` are what is left of the matrix from here on.
 template <int EL>
-__device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16], uint8_t *dst, long long stride, int rows, int cols, int wide, int lane, int add = 0) {
+__device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16], uint8_t *dst, long long stride, int rows, int cols, int wide, int lane) {
   uint4 *mine = reinterpret_cast<uint4 *>(turn + lane * 64);
 #pragma unroll
   for (int i = 0; i < 4; ++i) mine[i ^ ((lane >> 1) & 3)] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
@@ -540,16 +586,8 @@ __device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = i * 8 + (lane >> 2);
-      uint4 v = *reinterpret_cast<const uint4 *>(turn + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-      if (r < rows && c * (16 / EL) < cols) {
-        uint4 *to = reinterpret_cast<uint4 *>(dst + r * stride + c * 16);
-        if (EL == 4 && add) {
-          const float4 b = *reinterpret_cast<const float4 *>(to);
-          v = make_uint4(__float_as_uint(__uint_as_float(v.x) + b.x), __float_as_uint(__uint_as_float(v.y) + b.y),
-                         __float_as_uint(__uint_as_float(v.z) + b.z), __float_as_uint(__uint_as_float(v.w) + b.w));
-        }
-        *to = v;
-      }
+      const uint4 v = *reinterpret_cast<const uint4 *>(turn + r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+      if (r < rows && c * (16 / EL) < cols) *reinterpret_cast<uint4 *>(dst + r * stride + c * 16) = v;
     }
   } else {
     constexpr int PER = 64 / EL, RS = 32 / PER;      // elements of a row, rows a time
@@ -558,11 +596,7 @@ __device__ __forceinline__ void store_rows(uint8_t *turn, const uint32_t (&w)[16
       const uint8_t *src = turn + r * 64 + ((((c * EL) >> 4) ^ ((r >> 1) & 3)) << 4) + ((c * EL) & 15);
       if (c < cols) {
         if constexpr (EL == 2) *reinterpret_cast<uint16_t *>(dst + r * stride + c * 2) = *reinterpret_cast<const uint16_t *>(src);
-        else {
-          float *to = reinterpret_cast<float *>(dst + r * stride + c * 4);
-          const float v = *reinterpret_cast<const float *>(src);
-          *to = add ? v + *to : v;
-        }
+        else *reinterpret_cast<float *>(dst + r * stride + c * 4) = *reinterpret_cast<const float *>(src);
       }
     }
   }
@@ -651,29 +685,34 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     }
   } else if (warp == 1 && leader) {
     int s = 0, n = 0;
-    uint32_t ph = 0;
+    uint32_t ph = 0, used = 0;      // used: how often each accumulator has been, modulo two, a bit for each
     bool alive = true;
     const uint32_t hi = desc_hi(1024, 2), a_step = operand_step(g.r_mn), b_step = operand_step(g.c_mn);
     for (int t = tile0; t < g.n_tiles && alive; t += tile_step, ++n) {
-      const int buf = n & 1;
-      if (!mbar_wait_warp(acc_empty(buf), ((uint32_t)(n >> 1) & 1u) ^ 1u, abort_word, err, ERR_ACC_EMPTY)) break;
-      tc_fence_after();
-      const uint32_t d = tmem + (uint32_t)(buf * BN);
-      for (int k = 0; k < g.n_steps; ++k) {
-        if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
+      int k = 0;
+      for (int run = 0; run < g.runs && alive; ++run) {      // the first in one accumulator, the others in turn in the other: the next tile's first
+        const int buf = (n + (run > 0)) & 1;
+        if (!mbar_wait_warp(acc_empty(buf), ((used >> buf) & 1u) ^ 1u, abort_word, err, ERR_ACC_EMPTY)) { alive = false; break; }
+        used ^= 1u << buf;
         tc_fence_after();
-        const uint32_t st = base + (uint32_t)(s * P::STAGE);
-        const uint32_t a = operand_lo(st, g.r_mn), b = operand_lo(st + P::R_BYTES, g.c_mn);
-        if (elect_one()) {
+        const int first = k, last = run_start(g.n_steps, run + 1, g.runs);
+        const uint32_t d = tmem + (uint32_t)(buf * BN);
+        for (; k < last; ++k) {
+          if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
+          tc_fence_after();
+          const uint32_t st = base + (uint32_t)(s * P::STAGE);
+          const uint32_t a = operand_lo(st, g.r_mn), b = operand_lo(st + P::R_BYTES, g.c_mn);
+          if (elect_one()) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) umma<true, false>(d, a + (uint32_t)j * a_step, hi, b + (uint32_t)j * b_step, hi, g.idesc, (k > 0 || j > 0) ? 1u : 0u);
-          umma_commit<true>(empty(s), 3);
+            for (int j = 0; j < 4; ++j) umma<true, false>(d, a + (uint32_t)j * a_step, hi, b + (uint32_t)j * b_step, hi, g.idesc, (k > first || j > 0) ? 1u : 0u);
+            umma_commit<true>(empty(s), 3);
+          }
+          __syncwarp();
+          if (++s == P::STAGES) { s = 0; ph ^= 1u; }
         }
+        if (alive && elect_one()) umma_commit<true>(acc_full(buf), 3);
         __syncwarp();
-        if (++s == P::STAGES) { s = 0; ph ^= 1u; }
       }
-      if (alive && elect_one()) umma_commit<true>(acc_full(buf), 3);
-      __syncwarp();
     }
   } else if (warp >= 4) {
     const int ew = warp - 4, q = warp & 3, half = ew >> 2;
@@ -681,6 +720,8 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     float *bias = reinterpret_cast<float *>(base_ptr + P::OFF_BIAS + ew * BIAS_BYTES);
     const int n_blk = (o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK;
     int n = 0;
+    uint32_t used = 0;
+    bool alive = true;
     for (int t = tile0; t < g.n_tiles; t += tile_step, ++n) {
       int rt, ct;
       tile_at(g, t, rt, ct);
@@ -694,8 +735,22 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
         __syncwarp();
       }
-      if (!mbar_wait_warp(acc_full(buf), (uint32_t)(n >> 1) & 1u, abort_word, err, ERR_ACC_FULL)) break;
-      tc_fence_after();
+      for (int run = 0; run < g.runs; ++run) {
+        const int from = run > 0 ? buf ^ 1 : buf;
+        if (!mbar_wait_warp(acc_full(from), (used >> from) & 1u, abort_word, err, ERR_ACC_FULL)) { alive = false; break; }
+        used ^= 1u << from;
+        tc_fence_after();
+        if (run == 0) continue;
+        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
+#pragma unroll 1
+        for (int ch = 0; ch < BN / 64; ++ch)
+          if (rows > 0 && col0 + ch * 32 < o.cols) add_run(at + (uint32_t)(buf * BN + ch * 32), at + (uint32_t)(from * BN + ch * 32));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_rank0(acc_empty(from));
+      }
+      if (!alive) break;
 #pragma unroll 1
       for (int ch = 0; ch < BN / 64; ++ch) {
         const int c = col0 + ch * 32, cols = o.cols - c;
@@ -777,7 +832,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           for (int h = 0; h < 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(f[16 * h + i]);
-            store_rows<4>(turn, w, dst + h * 64, o.y_stride * 4, rows, cols - 16 * h, o.wide, lane, o.add);
+            store_rows<4>(turn, w, dst + h * 64, o.y_stride * 4, rows, cols - 16 * h, o.wide, lane);
           }
         } else {
 #pragma unroll
@@ -819,7 +874,7 @@ bool multiple(const void *p, long long stride, int el, int bytes) {
 
 Out out_of(const LinearProblem &p, int width) {      // width: columns of a vector access
   Out o;
-  o.rows = p.rows; o.cols = p.cols; o.act = p.act; o.layer = p.layer; o.bias_f32 = p.bias_f32; o.out_f32 = p.out_f32; o.add = p.add;
+  o.rows = p.rows; o.cols = p.cols; o.act = p.act; o.layer = p.layer; o.bias_f32 = p.bias_f32; o.out_f32 = p.out_f32;
   o.bias = p.bias; o.residual = p.residual; o.y = p.y; o.z = p.z; o.z8 = p.z8; o.z8_scale = p.z8_scale;
   o.residual_stride = p.residual_stride; o.y_stride = p.y_stride; o.z_stride = p.z_stride;
   const int el = p.out_f32 ? 4 : 2;
@@ -860,6 +915,7 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
   ClusterArgs g;
   g.n_steps = (p.red + BK - 1) / BK;
   g.n_rt = (p.rows + plan.tile_rows - 1) / plan.tile_rows;
+  g.run = steps_of_a_run(p);
   g.tile_rows = plan.tile_rows; g.stages = plan.stages; g.r_mn = p.r.mn; g.c_mn = p.c.mn;
   g.idesc = instruction(p.dtype, p.c.mn, p.r.mn, 128, plan.tile_rows);
   const int n_ct = (p.cols + BC - 1) / BC;
@@ -900,6 +956,7 @@ template <typename T, int ACT, int BN> cudaError_t launch_pair(const LinearProbl
   g.n_steps = (p.red + BK - 1) / BK;
   g.n_rt = (p.rows + PAIR_ROWS - 1) / PAIR_ROWS; g.n_ct = (p.cols + BN - 1) / BN;
   g.n_tiles = g.n_rt * g.n_ct;
+  g.runs = (g.n_steps + steps_of_a_run(p) - 1) / steps_of_a_run(p);
   g.band = band_of(p.red);
   g.r_mn = p.r.mn; g.c_mn = p.c.mn;
   g.idesc = instruction(p.dtype, p.r.mn, p.c.mn, PAIR_ROWS, BN);
@@ -982,32 +1039,13 @@ LinearPlan linear_plan(const LinearProblem &p) {
   return plan;
 }
 
-static cudaError_t launch_form(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
+cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
   *detail = "";
   if (plan.by_rows) return p.dtype == WINOCONV_F16 ? launch_rows<__half>(p, s) : launch_rows<__nv_bfloat16>(p, s);
   EncodeTiledFn enc = encode_tiled_fn();
   if (!enc) { *detail = "cuTensorMapEncodeTiled unavailable"; return cudaErrorNotSupported; }
   if (plan.pair) return p.dtype == WINOCONV_F16 ? launch_pair<__half>(p, plan.pair, enc, s, detail) : launch_pair<__nv_bfloat16>(p, plan.pair, enc, s, detail);
   return p.dtype == WINOCONV_F16 ? launch_cluster<__half>(p, plan, enc, s, detail) : launch_cluster<__nv_bfloat16>(p, plan, enc, s, detail);
-}
-
-// The tensor cores cut off what an fp32 accumulator has no place for, at every 16 values of the reduction: sums of one sign lose
-// 5e-5 of their value over 65536 values and 9e-4 over 2^20 (sums of both signs 1e-5 and 1.5e-4), which 16 bits do not show but f32 results
-// do.  These are added up over runs of 16384 values, a launch each (1e-5 and 3e-6 over any number).
-constexpr int RUN = 16384;
-cudaError_t launch_linear(const LinearProblem &p, const LinearPlan &plan, cudaStream_t s, const char **detail) {
-  if (!p.out_f32 || p.red <= RUN) return launch_form(p, plan, s, detail);
-  cudaError_t e = cudaSuccess;
-  for (int k = 0; k < p.red && e == cudaSuccess; k += RUN) {
-    LinearProblem q = p;
-    q.red = std::min(RUN, p.red - k);
-    q.add = k > 0;
-    auto from = [&](const MatOperand &m) { return MatOperand{(const uint16_t *)m.ptr + (m.mn ? (long long)k * m.stride : (long long)k), m.stride, m.mn}; };
-    q.r = from(p.r);
-    q.c = from(p.c);
-    e = launch_form(q, linear_plan(q), s, detail);
-  }
-  return e;
 }
 
 cudaError_t read_and_clear_linear_error(cudaStream_t s, unsigned int *code) {

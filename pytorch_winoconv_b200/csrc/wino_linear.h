@@ -20,7 +20,6 @@ struct LinearProblem {
   MatOperand r, c;
   int layer;                 // 1: z = product + bias, y = act(z) + residual; 0: y = product
   int act, bias_f32, out_f32;
-  int add;                   // (f32 results) y += product
   const void *bias;          // [cols] or null
   const void *residual;      // or null
   void *y, *z;               // z: pre-activation in dtype, or null

@@ -727,3 +727,84 @@ def test_activations_keep_their_relative_precision(act, dtype):
         dx, = torch.autograd.grad(lin.linear(leaf, w, activation=act), leaf, torch.full((len(z), cols), 1 / cols, dtype=dtype, device="cuda"))
         check(dx, slope, act, dtype, extra=size * off + floor + (0 if cols == 1 else 8 * half_step(slope / 8, dtype)))
     assert capi.read_device_error() == 0
+
+
+# ---- reductions longer than the tensor cores' accumulators are good for --------------------------------------------------
+def halves(rows, cols, seed, dtype, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.rand(rows, cols, device="cuda", generator=g).mul_(scale).to(dtype)
+
+
+# A run: 4096 values for float results, 16384 for f16 and 65536 for bf16.  An MMA adds 16 products to a sum; each of the 17 is cut off at
+# 2^-25 of the power of two that leads the largest (two bits below the sum's last place), so a sum that grows to S evenly loses at most
+# 17/2 x 2^-25 = 4.25 x 2^-24 of S for each 16 values (3.0 has been seen, of constant columns).  The runs are added in fp32, half a step
+# each: at most 256 of them here, 2^-16, and so are the eight parts of a cluster.
+def check_long(got, want):
+    run = {torch.float32: 4096, torch.float16: 16384, torch.bfloat16: 65536}[got.dtype]
+    long = run / 16 * 4.25 * 2.0 ** -24 + 2.0 ** -16
+    tol = want * long + (0 if got.dtype == torch.float32 else half_step(want, got.dtype) * (1 + long))
+    off = (got.double() - want).abs()
+    assert (off <= tol).all(), (off / want).max().item()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,k,n", [(2 ** 20, 40, 24), (2 ** 20 + 17, 72, 130), (2 ** 18, 1024, 1024), (2 ** 18 + 5, 515, 1030)])
+def test_weight_gradients_of_very_many_rows(rows, k, n, dtype):
+    """Sums of one sign, in clusters and in pairs, by vectors and by single values."""
+    x, gy = halves(rows, k, 1, dtype), halves(rows, n, 2, dtype, 2.0 ** -6)
+    want = torch.zeros(n, k, dtype=torch.float64, device="cuda")
+    for i in range(0, rows, 2 ** 16):
+        want += gy[i:i + 2 ** 16].double().t() @ x[i:i + 2 ** 16].double()
+    for w in (torch.zeros(n, k, dtype=dtype, device="cuda", requires_grad=True), torch.zeros(n, k, device="cuda", requires_grad=True)):
+        dw, = torch.autograd.grad(lin.linear(x, w), w, gy)
+        assert dw.dtype == w.dtype
+        check_long(dw, want)
+    assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 5, 40, 300, 2100])
+def test_very_many_features(rows, dtype):
+    """A long reduction in the forward pass and one in the data gradient."""
+    many, few = 262_152, 264
+    x, w = halves(rows, many, 1, dtype), halves(few, many, 2, dtype, 2.0 ** -4)
+    want = sum(x[:, i:i + 2 ** 16].double() @ w[:, i:i + 2 ** 16].double().t() for i in range(0, many, 2 ** 16))
+    check_long(lin.linear(x, w), want)
+    check_long(lin.linear(x, w, halves(1, few, 3, dtype)[0] * 0, activation="relu"), want)
+    w = w.t().contiguous()
+    leaf = halves(rows, few, 4, dtype).requires_grad_()
+    dx, = torch.autograd.grad(lin.linear(leaf, w), leaf, x)
+    check_long(dx, want)
+    assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows,k,n", [(33_000, 2048, 1024), (33_001, 1023, 2049), (70_000, 1024, 1024)])
+def test_float_weight_gradients_of_many_rows_in_pairs(rows, k, n):
+    """The same over runs in the pair kernel: exact where every sum is, and without the drift where it is not."""
+    x, gy = ints((rows, k), 1, 4, 0.25, torch.float16), ints((rows, n), 2, 4, 2.0 ** -6, torch.float16)
+    w = torch.zeros(n, k, device="cuda", requires_grad=True)
+    dw, = torch.autograd.grad(lin.linear(x, w), w, gy)
+    assert torch.equal(dw, (gy.double().t() @ x.double()).float())
+    x, gy = halves(rows, k, 1, torch.float16), halves(rows, n, 2, torch.float16)
+    dw, = torch.autograd.grad(lin.linear(x, w), w, gy)
+    check_long(dw, gy.double().t() @ x.double())
+    assert capi.read_device_error() == 0
+
+
+@gpu
+def test_the_longest_reduction():
+    """The most rows that the C ABI takes: a tile's sum takes about the second after which a wait gives up, none of its runs does."""
+    rows, dtype = (1 << 31) - 1152, torch.float16
+    v = torch.arange(1, 9, device="cuda").mul(2.0 ** -12).to(dtype)
+    x = v.expand(rows, 8).contiguous()
+    dw = torch.full((8, 8), float("nan"), dtype=dtype, device="cuda")
+    d = capi.LinearDesc(rows=rows, in_features=8, out_features=8, dtype=capi.F16)
+    capi.check(capi.lib().winoconv_linear_backward_weight(ctypes.byref(d), x.data_ptr(), 0, x.data_ptr(), dw.data_ptr(), capi.F16, torch.cuda.current_stream().cuda_stream),
+               "weight gradient")
+    assert capi.read_device_error() == 0
+    want = rows * torch.outer(v.double(), v.double())
+    # 2^14 runs to each of a cluster's eight parts: as many fp32 additions, off by 2^-24 at most of sums that are half the last one on average
+    assert ((dw.double() - want).abs() <= half_step(want, dtype) + want * (16384 / 16 * 4.25 * 2.0 ** -24 + 2.0 ** 14 * 2.0 ** -25)).all()
