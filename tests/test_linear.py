@@ -808,3 +808,38 @@ def test_the_longest_reduction():
     want = rows * torch.outer(v.double(), v.double())
     # 2^14 runs to each of a cluster's eight parts: as many fp32 additions, off by 2^-24 at most of sums that are half the last one on average
     assert ((dw.double() - want).abs() <= half_step(want, dtype) + want * (16384 / 16 * 4.25 * 2.0 ** -24 + 2.0 ** 14 * 2.0 ** -25)).all()
+
+
+# ---- the pair kernel's forms ---------------------------------------------------------------------------------------------
+# whole and odd widths with 256, 128 and 64 columns to a tile (the planner's choice for these sizes)
+PAIRS = [(2000, 64, 2000), (2001, 72, 1999), (1025, 520, 1000), (1500, 64, 1111), (900, 512, 1104), (700, 512, 1100), (509, 1000, 1531)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+@pytest.mark.parametrize("rows,k,n", PAIRS)
+def test_smooth_layers_of_many_rows(rows, k, n, act, pack, dtype):
+    """Each value of the result and of the gradients; z is exact, so what is kept of it is known too."""
+    x, w, b, r = make(rows, k, n, dtype, 11)
+    gy = ints((rows, n), 9, 4, 2.0 ** -3, dtype)
+    for t in (x, w, b, r):
+        t.requires_grad_()
+    y = lin.linear(x, w, b, r, activation=act, checkpoint=pack)
+    dx, dw, db, dr = torch.autograd.grad(y, (x, w, b, r), gy)
+    xd, wd, rd = (t.detach().double() for t in (x, w, r))
+    z = forward64(xd, wd, b.detach(), None, None)[0]
+    value, _, _, off = smooth64(z, act)
+    # the sum with the residual is rounded in fp32 before the result's type
+    check(y.detach(), value + rd, act, dtype, extra=value.abs() * off + 2.0 ** -120 + (value + rd).abs() * 2.0 ** -24)
+    kept_z, kept_x = (values8(z, dtype), values8(xd, dtype)) if pack else (z.to(dtype).double(), xd)
+    _, slope, size, off = smooth64(kept_z, act)
+    dz, gd = slope * gy.double(), gy.double().abs()
+    raw = gd * (size * off + 2.0 ** -120)                                   # of a value of dz before its rounding
+    tol_dz, sums = raw + half_step(dz, dtype) + raw * torch.finfo(dtype).eps, 2.0 ** -23
+    check(dx, dz @ wd, act, dtype, extra=tol_dz @ wd.abs() + (dz.abs() @ wd.abs()) * (n / 16 + 8) * sums)
+    check(dw, dz.t() @ kept_x, act, dtype, extra=tol_dz.t() @ kept_x.abs() + (dz.abs().t() @ kept_x.abs()) * (rows / 16 + 8) * sums)
+    check(db, dz.sum(0), act, dtype, extra=raw.sum(0) + dz.abs().sum(0) * (rows / 8 + 16) * sums)
+    assert torch.equal(dr, gy)
+    assert capi.read_device_error() == 0
