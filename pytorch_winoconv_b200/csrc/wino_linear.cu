@@ -973,7 +973,10 @@ template <typename T, int ACT, int BN> cudaError_t launch_pair(const LinearProbl
   return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 8), g);
 }
 template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
-  return bn == 256 ? launch_pair<T, ACT, 256>(p, enc, s, detail) : bn == 128 ? launch_pair<T, ACT, 128>(p, enc, s, detail) : launch_pair<T, ACT, 64>(p, enc, s, detail);
+  if constexpr (ACT >= 0) {      // (a product alone has columns that come in 64s, half a tile: linear_plan)
+    if (bn == 64) return launch_pair<T, ACT, 64>(p, enc, s, detail);
+  }
+  return bn == 256 ? launch_pair<T, ACT, 256>(p, enc, s, detail) : launch_pair<T, ACT, 128>(p, enc, s, detail);
 }
 template <typename T> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
   if (!p.layer) return launch_pair<T, -1>(p, bn, enc, s, detail);
