@@ -214,8 +214,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     // numbered by the tensors among the arguments of apply
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = layer[HAS_BIAS] && ctx->needs_input_grad(2),
                nr = layer[HAS_RESIDUAL] && ctx->needs_input_grad(2 + layer[HAS_BIAS]);
-    const at::Tensor &gy = grads[0];
-    c10::cuda::CUDAGuard guard(gy.device());
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const at::Tensor gy = grads[0].resolve_neg();
     if (nr) out[3] = gy;
     if (!nx && !nw && !nb) return out;
     const int64_t n = layer[OUT], k = layer[IN];
@@ -296,6 +296,10 @@ at::Tensor linear_call(const at::Tensor &x, const at::Tensor &weight, const std:
   check_eager("linear", {&x, &weight});
   if (bias) check_eager("linear", {&*bias});
   if (residual) check_eager("linear", {&*residual});
+  if (x.is_neg() || weight.is_neg() || (bias && bias->is_neg()) || (residual && residual->is_neg())) {      // memory that holds minus the values
+    auto of = [](const std::optional<at::Tensor> &t) { return t ? std::optional<at::Tensor>(t->resolve_neg()) : t; };
+    return linear_call(x.resolve_neg(), weight.resolve_neg(), of(bias), of(residual), act, pack);
+  }
   TORCH_CHECK(x.is_cuda(), "linear runs on CUDA devices only: there is no CPU path");
   TORCH_CHECK(is16(x), "linear: x must be float16 or bfloat16, got ", x.scalar_type());
   TORCH_CHECK(weight.dim() == 2, "linear: weight must be [out_features, in_features], got ", weight.sizes());
@@ -332,7 +336,7 @@ std::tuple<at::Tensor, at::Tensor> e4m3_pack(const at::Tensor &x_in) {
   at::AutoDispatchBelowADInplaceOrView no_graph;
   c10::cuda::CUDAGuard guard(x_in.device());
   const int64_t cols = x_in.size(-1);
-  const at::Tensor x = with_rows(as_rows(x_in, cols));
+  const at::Tensor x = with_rows(as_rows(x_in.resolve_neg(), cols));
   std::vector<int64_t> sizes(x_in.sizes().begin(), x_in.sizes().end());
   at::Tensor q = at::empty(sizes, plain(x).dtype(at::kFloat8_e4m3fn));
   sizes.back() = (cols + 31) / 32;

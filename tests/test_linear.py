@@ -843,3 +843,23 @@ def test_smooth_layers_of_many_rows(rows, k, n, act, pack, dtype):
     check(db, dz.sum(0), act, dtype, extra=raw.sum(0) + dz.abs().sum(0) * (rows / 8 + 16) * sums)
     assert torch.equal(dr, gy)
     assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1, 40])
+def test_lazily_negated_tensors(rows):
+    """Tensors whose memory holds minus their values (the imaginary part of a conjugate is one) give what their copies give."""
+    x, w, b, r = make(rows, 40, 24, torch.float16)
+    gy = ints((rows, 24), 9, 4, 2.0 ** -6, torch.float16)
+    part = torch.view_as_complex(torch.stack([torch.zeros_like(x), x], -1)).conj().imag
+    assert part.is_neg() and torch.equal(part, -x)
+    assert torch.equal(lin.linear(part, w, b, r), lin.linear(-x, w, b, r))
+    turned = torch._neg_view
+    assert torch.equal(lin.linear(x, turned(w), turned(b), turned(r)), lin.linear(x, -w, -b, -r))
+    leaves = [t.requires_grad_() for t in (x, w, b, r)]
+    got = torch.autograd.grad(lin.linear(turned(x), turned(w), b, r, activation="silu", checkpoint="e4m3"), leaves, turned(gy))
+    want = torch.autograd.grad(lin.linear(-x, -w, b, r, activation="silu", checkpoint="e4m3"), leaves, -gy)
+    assert all(torch.equal(i, j) for i, j in zip(got, want))
+    with torch.no_grad():
+        q, scale = checkpoint.pack(turned(x))
+        assert torch.equal(checkpoint.unpack(q, scale, x.dtype), -checkpoint.unpack(*checkpoint.pack(x), x.dtype))
