@@ -104,9 +104,12 @@ __device__ __forceinline__ uint32_t operand_step(int mn) { return mn ? 128u : 2u
 // result's type allows: at worst 4.6e-5 in f32 results, 1.8e-4 in f16 (half a step: 2.4e-4 to 4.9e-4), 7.3e-4 in bf16 (2.0e-3 to
 // 3.9e-3).  No wait lasts longer than a run, however long the reduction.
 constexpr int RUN_F32 = 4096 / BK, RUN_F16 = 16384 / BK, RUN_BF16 = 65536 / BK;      // steps
-int steps_of_a_run(const LinearProblem &p) { return p.out_f32 ? RUN_F32 : p.dtype == WINOCONV_F16 ? RUN_F16 : RUN_BF16; }
-// The step at which run `r` of `runs` starts.
-__device__ __forceinline__ int run_start(int steps, int r, int runs) { return (int)((long long)steps * r / runs); }
+int longest_run(const LinearProblem &p) { return p.out_f32 ? RUN_F32 : p.dtype == WINOCONV_F16 ? RUN_F16 : RUN_BF16; }
+// Steps of each run but the last where `steps` are shared out evenly to runs of `longest` at most.
+__host__ __device__ __forceinline__ int run_of(int steps, int longest) {
+  const int runs = (steps + longest - 1) / longest;
+  return (steps + runs - 1) / runs;
+}
 // 32 lanes x 32 columns of `sum` plus those of `run`.
 __device__ __forceinline__ void add_run(uint32_t sum, uint32_t run) {
   uint32_t a[32], b[32];
@@ -260,7 +263,7 @@ template <int S, bool WIDE> __device__ __forceinline__ void add_parts(uint32_t s
 }
 
 struct ClusterArgs {
-  int n_steps, run, n_rt, tile_rows, stages, r_mn, c_mn;
+  int n_steps, longest_run, n_rt, tile_rows, stages, r_mn, c_mn;
   uint32_t idesc;
 };
 
@@ -289,7 +292,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
   const int tile = (int)blockIdx.x / split, ct = tile / g.n_rt, rt = tile - ct * g.n_rt;      // CTAs in flight share columns: the weights are read once
   const int row0 = rt * g.tile_rows, col0 = ct * BC;
   const int k0 = (int)((long long)g.n_steps * part / split), k1 = (int)((long long)g.n_steps * (part + 1) / split);
-  const int steps = k1 - k0, runs = (steps + g.run - 1) / g.run;
+  const int run_steps = run_of(k1 - k0, g.longest_run), runs = (k1 - k0 + run_steps - 1) / run_steps;
   uint32_t acc_cols = 32;
   while (acc_cols < (uint32_t)g.tile_rows) acc_cols *= 2;
   const uint32_t tmem_cols = runs > 1 ? 2u * acc_cols : acc_cols;
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS, 2)
         if (!mbar_wait_warp(run_free, (uint32_t)(run - 1) & 1u, abort_word, err, ERR_ACC_EMPTY)) { alive = false; break; }
         tc_fence_after();
       }
-      const int first = k, last = k0 + run_start(steps, run + 1, runs);
+      const int first = k, last = min(k + run_steps, k1);
       const uint32_t d = run > 0 ? tmem + acc_cols : tmem;
       for (; k < last; ++k) {
         if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
@@ -559,7 +562,7 @@ template <int BN> struct PairTile {
 };
 
 struct PairArgs {
-  int n_steps, runs, n_rt, n_ct, n_tiles, band, r_mn, c_mn;
+  int n_steps, run_steps, runs, n_rt, n_ct, n_tiles, band, r_mn, c_mn;
   uint32_t idesc;
 };
 // Tiles are walked in bands of tile rows, column by column: the pairs at work at one time share few rows and few columns, which then
@@ -619,8 +622,9 @@ __device__ __forceinline__ void load_rows(uint8_t *turn, uint32_t (&w)[16], cons
   __syncwarp();
 }
 
-// ACT: the activation of a layer; -1: the product alone.
-template <typename T, int ACT, int BN>
+// ACT: the activation of a layer; -1: the product alone.  LONG: a reduction of several runs, with any activation where it is a layer.  (A
+// kernel of its own: the runs in the epilogue's loop over tiles cost the others up to 2 %, 8192 x 256 x 8192 72.0 us instead of 70.5.)
+template <typename T, int ACT, int BN, bool LONG>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
     pair_kernel(const __grid_constant__ CUtensorMap map_r, const __grid_constant__ CUtensorMap map_c, const __grid_constant__ Out o,
                 const __grid_constant__ PairArgs g) {
@@ -695,7 +699,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         if (!mbar_wait_warp(acc_empty(buf), ((used >> buf) & 1u) ^ 1u, abort_word, err, ERR_ACC_EMPTY)) { alive = false; break; }
         used ^= 1u << buf;
         tc_fence_after();
-        const int first = k, last = run_start(g.n_steps, run + 1, g.runs);
+        const int first = k, last = min(k + g.run_steps, g.n_steps);
         const uint32_t d = tmem + (uint32_t)(buf * BN);
         for (; k < last; ++k) {
           if (!mbar_wait_warp(full(s), ph, abort_word, err, ERR_FULL)) { alive = false; break; }
@@ -720,8 +724,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
     float *bias = reinterpret_cast<float *>(base_ptr + P::OFF_BIAS + ew * BIAS_BYTES);
     const int n_blk = (o.cols + e4m3::BLOCK - 1) / e4m3::BLOCK;
     int n = 0;
-    uint32_t used = 0;
-    bool alive = true;
+    [[maybe_unused]] uint32_t used = 0;
     for (int t = tile0; t < g.n_tiles; t += tile_step, ++n) {
       int rt, ct;
       tile_at(g, t, rt, ct);
@@ -735,22 +738,27 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
         }
         __syncwarp();
       }
-      for (int run = 0; run < g.runs; ++run) {
-        const int from = run > 0 ? buf ^ 1 : buf;
-        if (!mbar_wait_warp(acc_full(from), (used >> from) & 1u, abort_word, err, ERR_ACC_FULL)) { alive = false; break; }
-        used ^= 1u << from;
-        tc_fence_after();
-        if (run == 0) continue;
-        const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
+      if (!mbar_wait_warp(acc_full(buf), LONG ? (used >> buf) & 1u : (uint32_t)(n >> 1) & 1u, abort_word, err, ERR_ACC_FULL)) break;
+      tc_fence_after();
+      if constexpr (LONG) {
+        used ^= 1u << buf;
+        bool alive = true;
+        for (int run = 1; run < g.runs && alive; ++run) {      // the other accumulator into this one
+          const int from = buf ^ 1;
+          alive = mbar_wait_warp(acc_full(from), (used >> from) & 1u, abort_word, err, ERR_ACC_FULL);
+          used ^= 1u << from;
+          tc_fence_after();
+          const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(half * (BN / 2));
 #pragma unroll 1
-        for (int ch = 0; ch < BN / 64; ++ch)
-          if (rows > 0 && col0 + ch * 32 < o.cols) add_run(at + (uint32_t)(buf * BN + ch * 32), at + (uint32_t)(from * BN + ch * 32));
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_rank0(acc_empty(from));
+          for (int ch = 0; ch < BN / 64 && alive; ++ch)
+            if (rows > 0 && col0 + ch * 32 < o.cols) add_run(at + (uint32_t)(buf * BN + ch * 32), at + (uint32_t)(from * BN + ch * 32));
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_rank0(acc_empty(from));
+        }
+        if (!alive) break;
       }
-      if (!alive) break;
 #pragma unroll 1
       for (int ch = 0; ch < BN / 64; ++ch) {
         const int c = col0 + ch * 32, cols = o.cols - c;
@@ -814,7 +822,7 @@ __global__ void __launch_bounds__(PAIR_THREADS, 1)
           }
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            const act::F2 y = act::apply(act::F2(f[i], f[i + 1]), ACT);
+            const act::F2 y = act::apply(act::F2(f[i], f[i + 1]), LONG ? o.act : ACT);
             f[i] = y.lo(); f[i + 1] = y.hi();
           }
           if (o.residual) {
@@ -915,7 +923,7 @@ cudaError_t launch_cluster(const LinearProblem &p, const LinearPlan &plan, Encod
   ClusterArgs g;
   g.n_steps = (p.red + BK - 1) / BK;
   g.n_rt = (p.rows + plan.tile_rows - 1) / plan.tile_rows;
-  g.run = steps_of_a_run(p);
+  g.longest_run = longest_run(p);
   g.tile_rows = plan.tile_rows; g.stages = plan.stages; g.r_mn = p.r.mn; g.c_mn = p.c.mn;
   g.idesc = instruction(p.dtype, p.c.mn, p.r.mn, 128, plan.tile_rows);
   const int n_ct = (p.cols + BC - 1) / BC;
@@ -943,20 +951,21 @@ template <typename T> cudaError_t launch_rows(const LinearProblem &p, cudaStream
   return cudaLaunchKernelEx(&cfg, kern, (const T *)p.r.ptr, p.r.stride, (const T *)p.c.ptr, p.c.stride, p.red, out_of(p, 1));
 }
 
-template <typename T, int ACT, int BN> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+template <typename T, int ACT, int BN, bool LONG> cudaError_t launch_pair(const LinearProblem &p, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
   CUtensorMap mr, mc;
   if (!operand_map(&mr, enc, p.dtype, p.r, p.rows, p.red, 128) || !operand_map(&mc, enc, p.dtype, p.c, p.cols, p.red, BN / 2)) {
     *detail = "cuTensorMapEncodeTiled failed";
     return cudaErrorInvalidValue;
   }
-  auto kern = pair_kernel<T, ACT, BN>;
+  auto kern = pair_kernel<T, ACT, BN, LONG>;
   cudaError_t e = allow_smem((const void *)kern);
   if (e != cudaSuccess) return e;
   PairArgs g;
   g.n_steps = (p.red + BK - 1) / BK;
   g.n_rt = (p.rows + PAIR_ROWS - 1) / PAIR_ROWS; g.n_ct = (p.cols + BN - 1) / BN;
   g.n_tiles = g.n_rt * g.n_ct;
-  g.runs = (g.n_steps + steps_of_a_run(p) - 1) / steps_of_a_run(p);
+  g.run_steps = run_of(g.n_steps, longest_run(p));
+  g.runs = (g.n_steps + g.run_steps - 1) / g.run_steps;
   g.band = band_of(p.red);
   g.r_mn = p.r.mn; g.c_mn = p.c.mn;
   g.idesc = instruction(p.dtype, p.r.mn, p.c.mn, PAIR_ROWS, BN);
@@ -972,13 +981,18 @@ template <typename T, int ACT, int BN> cudaError_t launch_pair(const LinearProbl
   cfg.gridDim = dim3(2u * (unsigned)std::min(g.n_tiles, SMS / 2));
   return cudaLaunchKernelEx(&cfg, kern, mr, mc, out_of(p, 8), g);
 }
+bool is_long(const LinearProblem &p) { return (p.red + BK - 1) / BK > longest_run(p); }
 template <typename T, int ACT> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
   if constexpr (ACT >= 0) {      // (a product alone has columns that come in 64s, half a tile: linear_plan)
-    if (bn == 64) return launch_pair<T, ACT, 64>(p, enc, s, detail);
+    if (bn == 64) return launch_pair<T, ACT, 64, false>(p, enc, s, detail);
   }
-  return bn == 256 ? launch_pair<T, ACT, 256>(p, enc, s, detail) : launch_pair<T, ACT, 128>(p, enc, s, detail);
+  return bn == 256 ? launch_pair<T, ACT, 256, false>(p, enc, s, detail) : launch_pair<T, ACT, 128, false>(p, enc, s, detail);
+}
+template <typename T, int ACT> cudaError_t launch_pair_long(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  return bn == 256 ? launch_pair<T, ACT, 256, true>(p, enc, s, detail) : launch_pair<T, ACT, 128, true>(p, enc, s, detail);
 }
 template <typename T> cudaError_t launch_pair(const LinearProblem &p, int bn, EncodeTiledFn enc, cudaStream_t s, const char **detail) {
+  if (is_long(p)) return p.layer ? launch_pair_long<T, WINOCONV_ACT_NONE>(p, bn, enc, s, detail) : launch_pair_long<T, -1>(p, bn, enc, s, detail);
   if (!p.layer) return launch_pair<T, -1>(p, bn, enc, s, detail);
   switch (p.act) {
     case WINOCONV_ACT_RELU: return launch_pair<T, WINOCONV_ACT_RELU>(p, bn, enc, s, detail);
@@ -1009,7 +1023,7 @@ LinearPlan linear_plan(const LinearProblem &p) {
   // pairs: a step's time is the tensor pipe's for 256 columns, below that the L2's (24 and 20 KB a CTA at 14.5 TB/s in all)
   const struct { int bn; double step; } pairs[3] = {{256, 0.33}, {128, 0.20}, {64, 0.18}};
   for (const auto &q : pairs) {
-    if (q.bn == 64 && p.c.mn) continue;      // an MN-major operand comes in 64s: a CTA's half would be 32
+    if (q.bn == 64 && (p.c.mn || is_long(p))) continue;      // an MN-major operand comes in 64s: a CTA's half would be 32; long ones are built for 128 and more
     const double t = std::max(memory, 3.5 + (double)over(over(p.rows, PAIR_ROWS) * over(p.cols, q.bn), SMS / 2) * (n_steps * q.step + 0.3));
     if (plan.pair == 0 || t < best) {
       best = t;

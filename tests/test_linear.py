@@ -863,3 +863,25 @@ def test_lazily_negated_tensors(rows):
     with torch.no_grad():
         q, scale = checkpoint.pack(turned(x))
         assert torch.equal(checkpoint.unpack(q, scale, x.dtype), -checkpoint.unpack(*checkpoint.pack(x), x.dtype))
+
+
+@gpu
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+@pytest.mark.parametrize("rows,k,n", [(2048, 20_000, 2048), (2001, 20_000, 1999), (2304, 20_000, 1000), (1500, 20_000, 1111), (600, 20_000, 1100)])
+def test_layers_with_a_long_reduction(rows, k, n, pack):
+    """More than one run (f16), in pairs with 256 and 128 columns and in clusters: the whole epilogue, with sums that are exact."""
+    dtype = torch.float16
+    x, w, b, r = make(rows, k, n, dtype, 13)
+    z = forward64(x, w, b, None, None)[0]
+    for act in (None, "relu", "gelu", "gelu_tanh", "silu"):
+        w.requires_grad_(act == "relu")
+        y = lin.linear(x, w, b, r, activation=act, checkpoint=pack)
+        want = act64(z, act) + r.double()
+        off = 0 if act in (None, "relu") else smooth64(z, act)[3]
+        check(y.detach(), want, act, dtype, extra=None if act in (None, "relu") else act64(z, act).abs() * off + want.abs() * 2.0 ** -24 + 2.0 ** -120)
+        if act == "relu":      # through what was kept of z
+            gy = ints((rows, n), 9, 4, 2.0 ** -6, dtype)
+            dw, = torch.autograd.grad(y, w, gy)
+            dz, kept = reference_backward(x, w.detach(), gy, z, act, dtype, pack)
+            assert torch.equal(dw, (dz.t() @ kept).to(dtype))
+    assert capi.read_device_error() == 0
