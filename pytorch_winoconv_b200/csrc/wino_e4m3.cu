@@ -486,8 +486,9 @@ cudaError_t launch_sign_apply(int dtype, const void *gy, const uint8_t *bits, lo
   return dtype == WINOCONV_F16 ? launch(sign_apply_kernel<__half>, blocks, s, (const __half *)gy, bits, (unsigned long long)n, (__half *)gx)
                                : launch(sign_apply_kernel<__nv_bfloat16>, blocks, s, (const __nv_bfloat16 *)gy, bits, (unsigned long long)n, (__nv_bfloat16 *)gx);
 }
-// Runs of rows: multiples of the 32 that a block has in flight, short enough for three waves of four blocks on every SM (so that
-// the last wave costs little; the partial sums stay below a tenth of what is read), at most 65535 of them.
+// Runs of rows: equal shares of 32 rows or a multiple of that on average (a block has 16 in flight), short enough for three waves of
+// four blocks on every SM, so that the last wave costs little, and at most 65535 of them.  A run's partial sums cost 8 bytes a column,
+// written and read, of 32 or more (from 33 rows on: two runs of 16 and 17) that are read of gy alone.
 int act_grad_chunks(long long rows, int cols) {
   const long long strips = (cols + 255) / 256, groups = (rows + 31) / 32;
   const long long per = std::max<long long>({1, groups * strips / (4 * 3 * 148), (groups + 65534) / 65535});

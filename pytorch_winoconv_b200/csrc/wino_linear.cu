@@ -7,7 +7,9 @@
 //     weight gradient  R = dz and C = x, both read down their columns     dW
 //
 // "Down its columns" is an MN-major operand of the MMA: TMA brings [reduction][64 rows] boxes as they lie, nothing is transposed
-// or copied.  No form needs scratch or atomics, and each gives the same bits every time.  Three forms, chosen by linear_plan:
+// for it.  The kernels need no scratch and no atomics and give the same bits every time.  (What TMA does not read has been copied before:
+// rows that do not start on 16 bytes and float weights by pad_rows_kernel, a W that comes transposed by torch.)  Three forms, chosen by
+// linear_plan:
 //
 //   row kernel      one or two rows: weights read once by plain loads, FMA                        (bound by HBM)
 //   cluster kernel  few rows, few tiles: 128 columns x up to 256 rows by a cluster of CTAs        (HBM, or the launch)
