@@ -203,8 +203,8 @@ struct LinearFn : public torch::autograd::Function<LinearFn> {
     torch::autograd::variable_list out(6);
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!at::GradMode::is_enabled(), "linear: the gradients are not differentiable again (create_graph=True)");
+    auto saved = ctx->get_saved_variables();      // (hooks on them may compute anew what was not kept, with graphs of their own)
     at::AutoDispatchBelowADInplaceOrView no_graph;
-    auto saved = ctx->get_saved_variables();
     const auto layer = ctx->saved_data["layer"].toIntVector();
     for (int i = 1; i < 3; ++i)      // dense, unless a hook on saved tensors has laid them out anew
       if (saved[i].defined()) saved[i] = saved[i].contiguous();

@@ -885,3 +885,34 @@ def test_layers_with_a_long_reduction(rows, k, n, pack):
             dz, kept = reference_backward(x, w.detach(), gy, z, act, dtype, pack)
             assert torch.equal(dw, (dz.t() @ kept).to(dtype))
     assert capi.read_device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("pack", [None, "e4m3"])
+def test_layers_that_are_computed_again_in_the_backward_pass(pack):
+    """torch.utils.checkpoint runs the forward pass again from within the backward pass of the layer that asks for its saved tensors first:
+    the gradients are those of the layers without it, with other operators between them and a float input before them."""
+    from torch.utils.checkpoint import checkpoint as again
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(torch.nn.LayerNorm(64), lin.Linear(64, 96, activation="gelu", checkpoint=pack), torch.nn.Tanh(),
+                              lin.Linear(96, 40, checkpoint=pack)).cuda()
+    x = torch.randn(30, 64, device="cuda", requires_grad=True)
+    gy = ints((30, 40), 1, 4, 2.0 ** -3, torch.float16)
+    names = [x, *net.parameters()]
+    want = torch.autograd.grad(net(x), names, gy)
+    for reentrant in (False, True):
+        for t in names:
+            t.grad = None
+        again(net, x, use_reentrant=reentrant).backward(gy)
+        assert all(torch.equal(t.grad, g) for t, g in zip(names, want))
+    hooked = []
+
+    def unpack(t):
+        with torch.enable_grad():      # (a backward pass runs without)
+            hooked.append((t.detach().float().requires_grad_() * 2).requires_grad)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y = net[1](x)
+    y.backward(torch.ones_like(y))
+    assert hooked and all(hooked)      # a hook's own operators are differentiable
