@@ -27,7 +27,8 @@ Backward (the reference left only traces of one: ``include/splitstrideone/split_
 
 A fused ReLU is differentiated through the stored output; the fused max-pool is forward only.  With ``checkpoint="e4m3"`` a 16-bit
 layer keeps its input in eight bits (and the ReLU as a bit for each value) instead of the tensors themselves: little more than half
-the memory, the result and the data gradient unchanged, the weight gradient that of an input rounded to four significant bits.
+the memory, the result and the data gradient unchanged, the weight gradient that of an input rounded to four significant bits, none of
+them differentiable again.
 ``groups != 1`` and dilation raise (the reference accepts ``groups`` and silently computes groups = 1), and so does a call that a
 tracer would record (``torch.jit.trace``, ``make_fx``, ``torch.export``) or that carries a forward-mode gradient.
 """

@@ -138,6 +138,7 @@ struct ConvFn : public torch::autograd::Function<ConvFn> {
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(2), nb = bias && ctx->needs_input_grad(3);
     std::vector<at::Tensor> g;
     if (saved.size() == 3) {
+      TORCH_CHECK(!at::GradMode::is_enabled(), "convolution: the gradients of a layer that keeps eight bits are not differentiable again (create_graph=True)");
       at::AutoDispatchBelowADInplaceOrView no_graph;
       c10::cuda::CUDAGuard guard(grads[0].device());
       const auto x_type = (at::ScalarType)ctx->saved_data["x_type"].toInt();

@@ -299,3 +299,31 @@ def test_recorded_calls_and_forward_mode_are_refused(device):
     with torch.autograd.forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="forward-mode"):
             checkpoint.pack(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@gpu
+def test_gradients_of_convolutions_in_eight_bits_are_not_differentiable_again():
+    """They would come back as constants, and a penalty on them would be left out of a loss without a word."""
+    layer = conv.Conv2d(8, 16, 3, activation="relu", checkpoint="e4m3").cuda()
+    x = torch.randn(2, 8, 9, 9, device="cuda", requires_grad=True)
+    with pytest.raises(RuntimeError, match="not differentiable again"):
+        torch.autograd.grad(layer(x).float().square().sum(), x, create_graph=True)
+
+
+@gpu
+@pytest.mark.parametrize("activation", [None, "relu"])
+def test_convolutions_computed_again_and_kept_on_the_host(activation):
+    from torch.utils.checkpoint import checkpoint as again
+    torch.manual_seed(0)
+    net = torch.nn.Sequential(conv.Conv2d(8, 40, 3, padding=1, activation=activation, checkpoint="e4m3"), torch.nn.Tanh(),
+                              conv.Conv2d(40, 12, 3, activation=activation, checkpoint="e4m3")).cuda()
+    x = torch.randn(3, 8, 11, 9, device="cuda", requires_grad=True)
+    names = [x, *net.parameters()]
+    want = torch.autograd.grad(net(x).float().square().sum(), names)
+    again(net, x, use_reentrant=False).float().square().sum().backward()
+    assert all(torch.equal(t.grad, g) for t, g in zip(names, want))
+    with torch.autograd.graph.save_on_cpu():
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(net(x).float().square().sum(), names), want))
+    crop = torch.randn(3, 12, 13, 14, device="cuda")[:, 2:10, 1:12, 3:12].requires_grad_()
+    whole = crop.detach().clone().requires_grad_()
+    assert torch.equal(*(torch.autograd.grad(net(t).float().square().sum(), t)[0] for t in (crop, whole)))
